@@ -117,8 +117,26 @@ def lib():
         L.ct2x_vocab_id.restype = C.c_int32
         L.ct2x_vocab_id.argtypes = [C.c_void_p, C.c_int, C.c_char_p]
         L.ct2x_vocab_size.argtypes = [C.c_void_p, C.c_int]
+    if hasattr(L, "ct2x_attention_tree"):
+        _declare_cache_ops(L)
     _lib = L
     return L
+
+
+def _declare_cache_ops(L):
+    """Argument types of the attention over a serving cache (include/ct2_mi355.h)."""
+    P, N, I, F = C.c_void_p, C.c_int64, C.c_int, C.c_float
+    for name, args in {
+        "ct2x_attention_tree": [P, P, P, I, P, N, P, N, N, N, N, N, N, F, P, P, N, P],
+        "ct2x_attention_accumulate": [P, P, P, I, P, N, N, N, N, N, N, F, P, P, P, N, P],
+        "ct2x_cache_evict": [P, P, I, P, P, N, N, N, N, N, N, N, N, P, P, P, P, P, P],
+        "ct2x_cache_block_bounds": [P, I, P, P, N, N, N, N, N, N, P, P],
+        "ct2x_attention_blocks": [P, P, P, I, P, P, N, N, N, N, N, N, N, N, N, N, F, P, P, P, N, P],
+    }.items():
+        getattr(L, name).argtypes = args
+    for name, sizes in (("tree", 6), ("accumulate", 5), ("blocks", 7)):
+        f = getattr(L, "ct2x_attention_%s_scratch_bytes" % name)
+        f.restype, f.argtypes = N, [N] * sizes
 
 
 def check(rc):

@@ -530,6 +530,89 @@ int ct2x_attention_full_half(const float* d_q, const float* d_k, const float* d_
                              int64_t q_offset, float scale, int compute_kind, float* d_out,
                              void* stream);
 
+/* ---- attention over a serving cache ---------------------------------------------------------
+ * A long context that is read by many decode steps: several drafted tokens verified at once, a cache
+ * that keeps what was looked at, attention that reads a part of it. No counterpart in the reference.
+ *
+ * All of them work on K / V caches [batch, heads_kv, t_max, dhead] of kv_dtype (CT2X_F32 / CT2X_F16 /
+ * CT2X_BF16; values as raw 2-byte data) with fp32 queries and outputs. dhead is a multiple of 8 up to
+ * 256, heads a multiple of heads_kv (head h reads head h / (heads / heads_kv) of the cache), t_max *
+ * dhead * 4 < 2^31; tensors are aligned to 16 bytes. Entry b has d_lengths[b] committed positions
+ * (clamped to what the cache holds), or `length` where d_lengths is NULL (`length` is not read
+ * otherwise). What lies behind an entry's positions is never looked at: it may hold anything.
+ * Scores, softmax statistics and sums are fp32, products of 16-bit caches enter the matrix cores with
+ * the fp32 operand as two 16-bit terms. A row that sees nothing gets an output of zero.
+ * d_scratch: at least the *_scratch_bytes() of the same sizes (-1: the sizes are refused, see
+ * ct2x_last_error), content irrelevant before and after; one call at a time may use it, calls on one
+ * stream may share it. Calls enqueue kernels only and may be captured into a graph. */
+
+/* A tree of drafted tokens verified in one pass. The committed positions 0 .. n-1 (n = the entry's
+ * length) are followed in the cache by the drafted tokens' keys and values at n .. n + tokens - 1;
+ * lengths are clamped to t_max - tokens. d_q, d_out [batch, tokens, heads, dhead]. Drafted token i
+ * sees every committed position, and drafted token j where bit j % 64 of word j / 64 of
+ * d_tree_mask[batch, tokens, ceil(tokens / 64)] (row i) is set - usually its ancestors and itself;
+ * any mask is legal, bits >= tokens are not read. d_tree_mask NULL: j <= i (a chain: one draft, or
+ * the next chunk of a prompt). tokens <= 1024. */
+int64_t ct2x_attention_tree_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t heads_kv,
+                                          int64_t dhead, int64_t t_max);
+int ct2x_attention_tree(const float* d_q, const void* d_k_cache, const void* d_v_cache, int kv_dtype,
+                        const int32_t* d_lengths, int64_t length, const uint64_t* d_tree_mask,
+                        int64_t batch, int64_t tokens, int64_t heads, int64_t heads_kv, int64_t dhead,
+                        int64_t t_max, float scale, float* d_out, void* d_scratch,
+                        int64_t scratch_bytes, void* stream);
+
+/* The attention of one decode step that leaves its probabilities behind: d_q, d_out [batch, heads,
+ * dhead]; d_weights [batch, heads_kv, t_max] fp32 gains, at every position the entry has, the sum of
+ * the probabilities that the heads of the group gave it (in the order of the heads). What
+ * ct2x_cache_evict goes by. */
+int64_t ct2x_attention_accumulate_scratch_bytes(int64_t batch, int64_t heads, int64_t heads_kv,
+                                                int64_t dhead, int64_t t_max);
+int ct2x_attention_accumulate(const float* d_q, const void* d_k_cache, const void* d_v_cache,
+                              int kv_dtype, const int32_t* d_lengths, int64_t length, int64_t batch,
+                              int64_t heads, int64_t heads_kv, int64_t dhead, int64_t t_max,
+                              float scale, float* d_weights, float* d_out, void* d_scratch,
+                              int64_t scratch_bytes, void* stream);
+
+/* Eviction from a cache by accumulated attention weight. Per (entry, head of the cache) with n
+ * positions: all stay where n <= budget; otherwise the `recent` newest and the budget - recent of the
+ * others with the largest d_weights [batch, heads_kv, t_max] (equal weights: the lower position;
+ * NaN counts as the largest). What stays keeps its order and moves to the front of d_k_out / d_v_out
+ * [batch, heads_kv, t_max_out, dhead] and d_weights_out [batch, heads_kv, t_max_out]; behind it the
+ * outputs are left as they were. d_positions [batch, heads_kv, budget] receives the positions that
+ * stayed, -1 behind the last, d_lengths_out [batch] the new lengths. In place where an output is its
+ * input (t_max_out == t_max then; d_lengths_out may be d_lengths always); any other overlap is
+ * refused. 0 <= recent <= budget, 1 <= budget <= t_max_out. */
+int ct2x_cache_evict(const void* d_k_cache, const void* d_v_cache, int kv_dtype, const float* d_weights,
+                     const int32_t* d_lengths, int64_t length, int64_t batch, int64_t heads_kv,
+                     int64_t dhead, int64_t t_max, int64_t budget, int64_t recent, int64_t t_max_out,
+                     void* d_k_out, void* d_v_out, float* d_weights_out, int32_t* d_positions,
+                     int32_t* d_lengths_out, void* stream);
+
+/* The bounds of blocks of `block` positions (a multiple of 16 up to 256): d_bounds [batch, heads_kv,
+ * ceil(t_max / block), 2, dhead] in kv_dtype = the smallest and the largest value of every key
+ * channel over the entry's positions in the block (a NaN key makes NaN bounds). Only blocks from
+ * position d_first[b] (NULL: 0) on are computed - after an append: the length before it -, the others
+ * and those behind the entry's end are left as they were. */
+int ct2x_cache_block_bounds(const void* d_k_cache, int kv_dtype, const int32_t* d_first,
+                            const int32_t* d_lengths, int64_t length, int64_t batch, int64_t heads_kv,
+                            int64_t dhead, int64_t t_max, int64_t block, void* d_bounds, void* stream);
+
+/* The attention of one decode step over selected blocks of the cache: d_q, d_out [batch, heads,
+ * dhead]. A block's score is max over the heads of the group of sum_d max(q_d min_d, q_d max_d) with
+ * d_bounds of ct2x_cache_block_bounds - no key of the block scores higher -, summed in float64. The
+ * first `sink` and the last `local` blocks of the entry are always taken, then the best of the others
+ * up to `top` in all (equal scores: the earlier block; NaN counts as the largest); entries of at most
+ * `top` blocks read them all. The heads of a group share the choice. d_selected [batch, heads_kv,
+ * top] (NULL: not wanted) receives the blocks in ascending order, -1 behind the last. scale > 0,
+ * sink + local <= top. */
+int64_t ct2x_attention_blocks_scratch_bytes(int64_t batch, int64_t heads, int64_t heads_kv,
+                                            int64_t dhead, int64_t t_max, int64_t block, int64_t top);
+int ct2x_attention_blocks(const float* d_q, const void* d_k_cache, const void* d_v_cache, int kv_dtype,
+                          const void* d_bounds, const int32_t* d_lengths, int64_t length, int64_t batch,
+                          int64_t heads, int64_t heads_kv, int64_t dhead, int64_t t_max, int64_t block,
+                          int64_t top, int64_t sink, int64_t local, float scale, float* d_out,
+                          int32_t* d_selected, void* d_scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- engine: ctranslate2::Translator / Generator ------------------------------- */
 
 /* models::Model::load + ReplicaPool ctor (src/models/model.cc:561-784,
