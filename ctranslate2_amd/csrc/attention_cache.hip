@@ -6,7 +6,28 @@
 // by exp(m - M), and parts of the cache join the same way. out = o / l; a row that sees nothing has
 // l = 0 and an output of zero. Positions that a row does not see never enter a sum, whatever they
 // hold.
+//
+// Matrix cores, no LDS on the way. A wave takes kStep positions and NT tiles of 16 rows:
+//   S^T = K Q^T   the key rows as they lie in memory are the A operand, rows of q the columns of B;
+//                 a lane then holds kLane consecutive positions of one row (its column), so that
+//                 the row's maximum and rescaling are the lane's own but for two lane swaps;
+//   O^T = V^T P^T P^T is that same register file: the position that a lane's element stands for is a
+//                 free choice of which key row went into which row of the A operand, and it is made so
+//                 that B's layout comes out. V^T's rows are channels: a lane loads W consecutive
+//                 channels of a position (256 bytes per 16 lanes) and MFMA number e takes the e-th of
+//                 each, so output row r of MFMA e is channel W r + e and nothing is transposed; the
+//                 16-bit types pair positions with one v_perm per register.
+// 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as two
+// 16-bit terms hi + lo, which leaves 2^-18 (bfloat16) / 2^-22 (float16) of them - the output is
+// float32, and one term would cost 2^-9. float32 caches use the float32 MFMA, nothing is rounded.
+//
+// Work is cut evenly whatever the lengths: the rounds (kStep positions per wave that shares a row
+// group) of all (entry, head, row group) units form one line, workgroup w of G takes the w-th G-th of
+// it. A unit that lies within one workgroup is finished there; the others leave (m, l, o) per part
+// and join_kernel adds them. A workgroup leaves at most two such parts (its first and its last unit).
 #include <hip/hip_fp16.h>
+
+#include <algorithm>
 
 #include "cache_ops.h"
 #include "device_utils.h"
@@ -16,141 +37,834 @@ namespace ct2x {
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float to_float(T x);
-template <>
-__device__ __forceinline__ float to_float(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_float(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+// Buffer offsets that are out of range of every head's region (at most 2^31 - 2^20 bytes), the load
+// returns zeros: of a row that is not there, and of channels behind dhead; their sum does not wrap.
+constexpr uint32_t kNoRow = 0x80000000u, kNoChannel = 0x7ff00000u;
 
-// One workgroup per (entry, row): the waves walk tiles of 64 positions, lane = position for the
-// scores, lane = channel for the outputs, and join in LDS.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void cache_attention_kernel(CacheAttnParams p) {
-  __shared__ float q_s[256];
-  __shared__ float m_s[4], l_s[4], o_s[4][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;  // ((b * tokens) + i) * heads + h
-  const int64_t h = row % p.heads, i = row / p.heads % p.tokens, b = row / p.heads / p.tokens;
-  const int64_t hkv = h / (p.heads / p.heads_kv);
-  const int dhead = static_cast<int>(p.dhead);
+constexpr int kF32 = 0, kF16 = 4, kBF16 = 5;
+
+// How a launch cuts its work; the same on the host and in every kernel of a call.
+struct CachePlan {
+  int row_waves;    // waves of a workgroup that take different rows; the others share rows and take
+                    // different positions
+  int unit_rows;    // rows of a unit
+  int row_groups;   // units per (entry, head of the cache)
+  int round_keys;   // positions of a round
+  int grid;         // workgroups at most
+  int min_rounds;   // per workgroup
+  bool whole;       // one workgroup per unit
+  int64_t score_pitch;  // accumulate: floats between the score rows
+  // scratch, in floats
+  int64_t parts_ml, parts_o, stats, scores, total;
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x)))) |
+         static_cast<int64_t>(uniform(static_cast<int>(x >> 32))) << 32;
+}
+
+__device__ __forceinline__ int committed(const CacheAttnParams& p, int64_t b) {
   const int64_t room = p.t_max - (p.view == CacheView::kTree ? p.tokens : 0);
-  int64_t len = p.lengths ? p.lengths[b] : p.length;
-  len = len < 0 ? 0 : (len > room ? room : len);
-  int64_t end = p.view == CacheView::kTree ? len + p.tokens : len;
-  if (p.view == CacheView::kBlocks) end = p.top * p.block;
-  for (int d = threadIdx.x; d < dhead; d += kThreads) q_s[d] = p.q[row * dhead + d];
-  __syncthreads();
-  const int64_t words = (p.tokens + 63) / 64;
-  const uint64_t* mask = p.mask ? p.mask + (b * p.tokens + i) * words : nullptr;
-  const int32_t* selected = p.selected ? p.selected + (b * p.heads_kv + hkv) * p.top : nullptr;
-  const T* k = static_cast<const T*>(p.k) + (b * p.heads_kv + hkv) * p.t_max * dhead;
-  const T* v = static_cast<const T*>(p.v) + (b * p.heads_kv + hkv) * p.t_max * dhead;
-  float* raw = p.weights ? static_cast<float*>(p.scratch) + (b * p.heads + h) * p.t_max : nullptr;
+  const int64_t n = p.lengths ? p.lengths[b] : p.length;
+  return static_cast<int>(n < 0 ? 0 : (n > room ? room : n));
+}
 
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t t0 = wave * 64; t0 < end; t0 += kThreads) {
-    int64_t t = t0 + lane;
-    bool visible = t < end;
-    if (p.view == CacheView::kBlocks) {
-      const int32_t j = visible ? selected[t / p.block] : -1;
-      t = j * p.block + t % p.block;
-      visible = j >= 0 && t < len;
-    } else if (p.view == CacheView::kTree && visible && t >= len) {
-      const int64_t j = t - len;
-      visible = mask ? (mask[j >> 6] >> (j & 63)) & 1 : j <= i;
-    }
-    float s = -INFINITY;
-    if (visible) {
-      float dot = 0.f;
-      for (int d = 0; d < dhead; ++d) dot = fmaf(q_s[d], to_float(k[t * dhead + d]), dot);
-      s = dot * p.scale;
-      if (raw) raw[t] = s;
-    }
-    const float top = fmaxf(m, wave_max(s));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float e = visible ? expf(s - base) : 0.f, keep = m == -INFINITY ? 0.f : expf(m - base);
-    l = l * keep + wave_sum(e);
-    for (int c = 0; c < 4; ++c) o[c] *= keep;
-    m = top;
-    for (int j = 0; j < 64; ++j) {
-      if (!__shfl(visible, j)) continue;
-      const float e_j = __shfl(e, j);
-      const int64_t t_j = __shfl(t, j);
-      for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < dhead) o[c] = fmaf(e_j, to_float(v[t_j * dhead + c * 64 + lane]), o[c]);
+// positions that entry b's rows walk (selected blocks: counted block by block)
+__device__ __forceinline__ int walked(const CacheAttnParams& p, int64_t b) {
+  const int n = committed(p, b);
+  if (p.view == CacheView::kTree) return n + static_cast<int>(p.tokens);
+  if (p.view == CacheView::kDense) return n;
+  const int64_t blocks = (n + p.block - 1) / p.block;
+  return static_cast<int>((blocks < p.top ? blocks : p.top) * p.block);
+}
+
+// at least one: an entry without positions still has outputs to write
+__device__ __forceinline__ int rounds_of(const CacheAttnParams& p, const CachePlan& plan, int64_t b) {
+  const int n = (walked(p, b) + plan.round_keys - 1) / plan.round_keys;
+  return n < 1 ? 1 : n;
+}
+
+// The line of all rounds: its length and how many workgroups share it.
+struct Line {
+  int64_t total;
+  int64_t groups;
+  __device__ __forceinline__ int64_t start(int64_t w) const { return w * total / groups; }
+};
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(static_cast<long long>(x), o, 64);
+  return x;
+}
+
+// rounds of the units of entries 0 .. entries - 1 (per unit of an entry: times units)
+__device__ __forceinline__ int64_t rounds_before(const CacheAttnParams& p, const CachePlan& plan, int64_t entries) {
+  int64_t sum = 0;
+  for (int64_t b = threadIdx.x & 63; b < entries; b += 64) sum += rounds_of(p, plan, b);
+  return uniform64(wave_sum64(sum)) * p.heads_kv * plan.row_groups;
+}
+
+__device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CachePlan& plan) {
+  Line line;
+  line.total = rounds_before(p, plan, p.batch);
+  const int64_t groups = line.total / plan.min_rounds;
+  line.groups = groups < 1 ? 1 : (groups > plan.grid ? plan.grid : groups);
+  return line;
+}
+
+// ---- the types -------------------------------------------------------------------------------
+
+template <int kType>
+struct Mfma {  // 16-bit
+  static __device__ __forceinline__ v4f mul(v4u a, v4u b, v4f c) {
+    if constexpr (kType == kF16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
+                                                     0);
+  }
+  // x = hi + lo up to half a step of lo, both pairs packed
+  static __device__ __forceinline__ void split(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    v2f x = {x0, x1};
+    if constexpr (kType == kF16) {
+      const v2h h = __builtin_convertvector(x, v2h);
+      hi = __builtin_bit_cast(uint32_t, h);
+      lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(x - __builtin_convertvector(h, v2f), v2h));
+    } else {
+      const v2bf h = __builtin_convertvector(x, v2bf);
+      hi = __builtin_bit_cast(uint32_t, h);
+      lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(x - __builtin_convertvector(h, v2f), v2bf));
     }
   }
-  if (lane == 0) {
-    m_s[wave] = m;
-    l_s[wave] = l;
-  }
-  for (int c = 0; c < 4; ++c) o_s[wave][c * 64 + lane] = o[c];
-  __syncthreads();
-  float top = -INFINITY, total = 0.f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, m_s[w]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float keep[4];
-  for (int w = 0; w < 4; ++w) {
-    keep[w] = m_s[w] == -INFINITY ? 0.f : expf(m_s[w] - base);
-    total += l_s[w] * keep[w];
-  }
-  const float inverse = total == 0.f ? 0.f : 1.f / total;
-  for (int d = threadIdx.x; d < dhead; d += kThreads) {
-    float sum = 0.f;
-    for (int w = 0; w < 4; ++w) sum += o_s[w][d] * keep[w];
-    p.out[row * dhead + d] = total == 0.f ? 0.f : sum * inverse;
-  }
-  if (raw) {  // the row's statistics wait behind the scores of all rows
-    float* stats = static_cast<float*>(p.scratch) + p.batch * p.heads * p.t_max + (b * p.heads + h) * 2;
-    if (threadIdx.x == 0) {
-      stats[0] = base;
-      stats[1] = inverse;
+};
+
+template <int kType>
+__device__ __forceinline__ float element(const void* base, int64_t i) {
+  if constexpr (kType == kF32) return static_cast<const float*>(base)[i];
+  else if constexpr (kType == kF16) return __half2float(static_cast<const __half*>(base)[i]);
+  else return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[i]) << 16);
+}
+
+// the larger / the sum over the four lanes of a row (lanes c, c + 16, c + 32, c + 48)
+__device__ __forceinline__ float rows_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+  x = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+  x = __int_as_float(a[0]) + __int_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+
+// exp2(m - base) of a running maximum that may still be -inf
+__device__ __forceinline__ float shift_of(float m, float base) { return __builtin_amdgcn_exp2f(m - base); }
+__device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <int kType, int DP, int NT>
+struct Tile {
+  static constexpr bool kHalf = kType != kF32;
+  static constexpr int kStep = kHalf ? 32 : 16;   // positions of a wave's step
+  static constexpr int kLane = kStep / 4;         // positions of a row that a lane holds
+  static constexpr int kBytes = kHalf ? 2 : 4;
+  static constexpr int kChunks = kHalf ? DP / 32 : DP / 16;  // K: loads of 16 bytes per key row and lane
+  static constexpr int kKeyTiles = kStep / 16;
+  static constexpr int W = kHalf ? (DP == 64 ? 4 : 8) : 4;  // V: channels of a load
+  static constexpr int H = DP / (16 * W);                    // V: loads per position and lane
+  static constexpr int E = H * W;                            // output tiles of 16 channels
+  static constexpr int kWords = W * kBytes / 4;              // registers of a V load
+};
+
+// ---- the kernel ------------------------------------------------------------------------------
+
+template <int kType, int DP, int NT, CacheView kView>
+struct Worker {
+  using T = Tile<kType, DP, NT>;
+  const CacheAttnParams& p;
+  const CachePlan& plan;
+  float* lds;  // 2 x NT x (E x 4 + 2) x 64 floats
+  int lane, g, c, wave_r, wave_k, key_waves;
+  int group, rows, row_bytes;
+  uint32_t k_channel[T::kChunks], v_channel[T::H];  // byte offsets of the lane's channels in a row
+
+  // the unit
+  int64_t b;
+  int hkv, row0;   // row0: first row of the wave
+  int len, end;    // committed positions, positions walked
+  const char *k_base, *v_base;
+  __amdgpu_buffer_rsrc_t k_rsrc, v_rsrc;
+  const int32_t* selected;
+  uint32_t block_magic;
+
+  uint32_t q_hi[NT][T::kChunks][4], q_lo[NT][T::kHalf ? T::kChunks : 1][4];
+  float factor[NT];
+  float m[NT], l[NT];
+  v4f o[NT][T::E];
+  v4u k[T::kKeyTiles][T::kChunks];
+  uint32_t v[T::kLane][T::H][T::kWords];
+
+  __device__ __forceinline__ Worker(const CacheAttnParams& p, const CachePlan& plan, float* lds)
+      : p(p), plan(plan), lds(lds) {
+    lane = threadIdx.x & 63;
+    g = lane >> 4;
+    c = lane & 15;
+    const int wave = uniform(threadIdx.x >> 6);
+    wave_r = wave % plan.row_waves;
+    wave_k = wave / plan.row_waves;
+    key_waves = kWaves / plan.row_waves;
+    group = static_cast<int>(p.heads / p.heads_kv);
+    rows = static_cast<int>(p.tokens) * group;
+    row_bytes = static_cast<int>(p.dhead) * T::kBytes;
+    if constexpr (kView == CacheView::kBlocks)
+      block_magic = static_cast<uint32_t>(((1ull << 32) + p.block / 16 - 1) / (p.block / 16));
+#pragma unroll
+    for (int s = 0; s < T::kChunks; ++s) {
+      const int byte = s * 64 + g * 16;
+      k_channel[s] = byte < row_bytes ? byte : kNoChannel;
     }
+#pragma unroll
+    for (int h = 0; h < T::H; ++h) {
+      const int byte = (h * 16 + c) * T::W * T::kBytes;
+      v_channel[h] = byte < row_bytes ? byte : kNoChannel;
+    }
+  }
+
+  // first element of a row's query and output
+  __device__ __forceinline__ int64_t row_at(int row) const {
+    const int i = row / group, h = row - i * group;
+    return ((b * p.tokens + i) * p.heads + hkv * group + h) * p.dhead;
+  }
+
+  __device__ __forceinline__ void begin(int64_t entry, int unit) {
+    b = entry;
+    hkv = unit / plan.row_groups;
+    row0 = (unit % plan.row_groups * plan.row_waves + wave_r) * NT * 16;
+    len = uniform(committed(p, b));
+    end = uniform(walked(p, b));
+    const int64_t head = b * p.heads_kv + hkv;
+    const int64_t offset = uniform64(head * p.t_max * row_bytes);
+    k_base = static_cast<const char*>(p.k) + offset;
+    v_base = static_cast<const char*>(p.v) + offset;
+    // the region that loads may reach: the entry's positions, nothing behind them
+    const int reach = (kView == CacheView::kTree ? end : len) * row_bytes;
+    k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(k_base), 0, reach, 0x00027000);
+    v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(v_base), 0, reach, 0x00027000);
+    if constexpr (kView == CacheView::kBlocks) selected = p.selected + uniform64(head * p.top);
+    load_queries();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int e = 0; e < T::E; ++e) o[n][e] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  __device__ __forceinline__ void load_queries() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + n * 16 + c;
+      const float* q = p.q + row_at(row < rows ? row : 0);
+      if constexpr (T::kHalf) {
+        float x[T::kChunks][8];
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < T::kChunks; ++s) {
+          const int d = s * 32 + g * 8;
+          const bool there = row < rows && d < p.dhead;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            v4f y = {0.f, 0.f, 0.f, 0.f};
+            if (there) y = *reinterpret_cast<const v4f*>(q + d + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[s][4 * i + j] = y[j];
+              most = fmaxf(most, fabsf(y[j]));
+            }
+          }
+        }
+        // to [1, 2) by a power of two, which the factor takes back: float16 has no room for less or more
+        const int power = ilogbf(fmaxf(rows_max(most), 1.17549435e-38f));
+        const int shift = power > 126 ? 126 : power;
+        factor[n] = p.scale * kLog2e * ldexpf(1.f, shift);
+        const float down = ldexpf(1.f, -shift);
+#pragma unroll
+        for (int s = 0; s < T::kChunks; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, q_hi[n][s][j], q_lo[n][s][j]);
+      } else {
+        factor[n] = p.scale * kLog2e;
+#pragma unroll
+        for (int s = 0; s < T::kChunks; ++s) {
+          const int d = s * 16 + g * 4;
+          v4f y = {0.f, 0.f, 0.f, 0.f};
+          if (row < rows && d < p.dhead) y = *reinterpret_cast<const v4f*>(q + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = __float_as_uint(y[j]);
+        }
+      }
+    }
+  }
+
+  // cache position of walked position t (a multiple of 4); negative: none
+  __device__ __forceinline__ int position(int t) const {
+    if constexpr (kView != CacheView::kBlocks) return t;
+    const uint32_t u = static_cast<uint32_t>(t) >> 4, j = __umulhi(u, block_magic);
+    const uint32_t j1 = block_magic == 0u ? u : j;  // blocks of 16: 2^32 / 1 does not fit the multiplier
+    if (t >= end) return -1;
+    const int at = selected[j1];
+    return at < 0 ? -1 : at * static_cast<int>(p.block) + t - static_cast<int>(j1) * static_cast<int>(p.block);
+  }
+
+  __device__ __forceinline__ uint32_t byte_of(int at) const {
+    return at < 0 ? kNoRow : static_cast<uint32_t>(at) * static_cast<uint32_t>(row_bytes);
+  }
+
+  // step: first walked position; negative: nothing to load (zeros)
+  __device__ __forceinline__ void load_keys(int step) {
+#pragma unroll
+    for (int i = 0; i < T::kKeyTiles; ++i) {
+      // row c of tile i is the position that the lanes' elements i * 4 .. i * 4 + 3 stand for
+      const int key = T::kHalf ? (c >> 2) * 8 + i * 4 : (c >> 2) * 4;
+      const int at = step < 0 ? -1 : position(step + key);
+      const uint32_t row = at < 0 ? kNoRow : byte_of(at + (c & 3));
+#pragma unroll
+      for (int s = 0; s < T::kChunks; ++s)
+        k[i][s] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, row + k_channel[s], 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void load_values(int step) {
+    const int at = step < 0 ? -1 : position(step + g * T::kLane);
+    const uint32_t row = byte_of(at);
+#pragma unroll
+    for (int j = 0; j < T::kLane; ++j)
+#pragma unroll
+      for (int h = 0; h < T::H; ++h) {
+        const uint32_t from = row + v_channel[h] + j * row_bytes;
+        if constexpr (T::kWords == 4) {
+          const v4u x = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, from, 0, 0);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[j][h][w] = x[w];
+        } else {
+          const v2u x = __builtin_amdgcn_raw_buffer_load_b64(v_rsrc, from, 0, 0);
+          v[j][h][0] = x[0];
+          v[j][h][1] = x[1];
+        }
+      }
+  }
+
+  // does row `row` see walked position t (at: its cache position)?
+  __device__ __forceinline__ bool sees(int row, int at) const {
+    if (at < 0) return false;
+    if (at < len) return true;
+    if (kView != CacheView::kTree || at >= end || row >= rows) return false;
+    const int j = at - len, i = row / group;
+    if (!p.mask) return j <= i;
+    const int words = (static_cast<int>(p.tokens) + 63) / 64;
+    return (p.mask[(b * p.tokens + i) * words + (j >> 6)] >> (j & 63)) & 1;
+  }
+
+  __device__ __forceinline__ bool values_finite() const {
+    bool fine = true;
+#pragma unroll
+    for (int j = 0; j < T::kLane; ++j)
+#pragma unroll
+      for (int h = 0; h < T::H; ++h)
+#pragma unroll
+        for (int w = 0; w < T::kWords; ++w) {
+          const uint32_t x = v[j][h][w];
+          if constexpr (kType == kF32) {
+            fine &= (x & 0x7f800000u) != 0x7f800000u;
+          } else {
+            constexpr uint32_t e = kType == kF16 ? 0x7c00u : 0x7f80u;
+            fine &= (x & e) != e && (x >> 16 & e) != e;
+          }
+        }
+    return fine;
+  }
+
+  // one step over positions step .. step + kStep - 1, whose keys and values are in registers or on
+  // their way; `next` is loaded as their registers come free
+  __device__ __forceinline__ void advance(int step, int next) {
+    float s[NT][T::kLane];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < T::kKeyTiles; ++i) {
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (T::kHalf) {
+#pragma unroll
+          for (int x = 0; x < T::kChunks; ++x) {
+            acc = Mfma<kType>::mul(k[i][x], v4u{q_hi[n][x][0], q_hi[n][x][1], q_hi[n][x][2], q_hi[n][x][3]}, acc);
+            acc = Mfma<kType>::mul(k[i][x], v4u{q_lo[n][x][0], q_lo[n][x][1], q_lo[n][x][2], q_lo[n][x][3]}, acc);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < T::kChunks; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][x][j]), __uint_as_float(q_hi[n][x][j]),
+                                                         acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][i * 4 + j] = acc[j] * factor[n];
+      }
+    }
+    load_keys(next);
+
+    const int at = position(step + g * T::kLane);
+    const bool full = __all(at >= 0 && at + T::kLane <= len);
+    uint32_t hidden[NT];  // bit j: the row does not see the lane's position j
+#pragma unroll
+    for (int n = 0; n < NT; ++n) hidden[n] = 0u;
+    if (!full) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < T::kLane; ++j)
+          if (!sees(row0 + n * 16 + c, at < 0 ? -1 : at + j)) {
+            s[n][j] = -INFINITY;
+            hidden[n] |= 1u << j;
+          }
+    }
+    if (kView == CacheView::kDense && p.weights) {
+      // the scores (times log2 e) wait for the row's statistics; the rows' pitch is a multiple of a step
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int row = row0 + n * 16 + c;
+        if (row < rows) {
+          float* to = static_cast<float*>(p.scratch) + plan.scores +
+                      ((b * p.heads_kv + hkv) * rows + row) * plan.score_pitch + step + g * T::kLane;
+#pragma unroll
+          for (int j = 0; j < T::kLane; j += 4)
+            *reinterpret_cast<v4f*>(to + j) = v4f{s[n][j], s[n][j + 1], s[n][j + 2], s[n][j + 3]};
+        }
+      }
+    }
+
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float most = s[n][0];
+#pragma unroll
+      for (int j = 1; j < T::kLane; ++j) most = fmaxf(most, s[n][j]);
+      most = fmaxf(m[n], rows_max(most));
+      const float base = finite_base(most);
+      if (__any(most > m[n])) {
+        const float keep = shift_of(m[n], base);
+        l[n] *= keep;
+#pragma unroll
+        for (int e = 0; e < T::E; ++e) o[n][e] *= keep;
+        m[n] = most;
+      }
+#pragma unroll
+      for (int j = 0; j < T::kLane; ++j) {
+        s[n][j] = __builtin_amdgcn_exp2f(s[n][j] - base);
+        l[n] += s[n][j];
+      }
+    }
+
+    if (kView == CacheView::kTree && !full && !__all(values_finite())) {
+      add_values_apart(step, s, hidden);
+    } else if constexpr (T::kHalf) {
+      v4u hi[NT], lo[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a, d;
+          Mfma<kType>::split(s[n][2 * j], s[n][2 * j + 1], a, d);
+          hi[n][j] = a;
+          lo[n][j] = d;
+        }
+#pragma unroll
+      for (int h = 0; h < T::H; ++h)
+#pragma unroll
+        for (int e = 0; e < T::W; ++e) {
+          v4u a;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            a[w] = __builtin_amdgcn_perm(v[2 * w + 1][h][e >> 1], v[2 * w][h][e >> 1],
+                                         e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) o[n][h * T::W + e] = Mfma<kType>::mul(a, hi[n], o[n][h * T::W + e]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) o[n][h * T::W + e] = Mfma<kType>::mul(a, lo[n], o[n][h * T::W + e]);
+        }
+    } else {
+#pragma unroll
+      for (int h = 0; h < T::H; ++h)
+#pragma unroll
+        for (int e = 0; e < T::W; ++e)
+#pragma unroll
+          for (int j = 0; j < T::kLane; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              o[n][h * T::W + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][h][e]), s[n][j],
+                                                                        o[n][h * T::W + e], 0, 0, 0);
+    }
+    load_values(next);
+  }
+
+  // A drafted position holds NaN or infinite values that some rows must not see: 0 x inf would reach
+  // them through the matrix cores, so this step is added on the vector pipe, row by row.
+  __device__ void add_values_apart(int step, const float (&s)[NT][T::kLane], const uint32_t (&hidden)[NT]) {
+#pragma unroll 1
+    for (int key = 0; key < T::kStep; ++key) {
+      const int at = step + key, from = key / T::kLane * 16 + c, j = key % T::kLane;
+      if (at >= end) break;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x = s[n][0];
+#pragma unroll
+        for (int i = 1; i < T::kLane; ++i) x = j == i ? s[n][i] : x;
+        x = __shfl(x, from);
+        const bool seen = !(__shfl(hidden[n], from) >> j & 1);
+#pragma unroll
+        for (int h = 0; h < T::H; ++h)
+#pragma unroll
+          for (int e = 0; e < T::W; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int d = (h * 16 + g * 4 + i) * T::W + e;
+              if (seen && d < p.dhead)
+                o[n][h * T::W + e][i] = fmaf(x, element<kType>(v_base, static_cast<int64_t>(at) * p.dhead + d),
+                                             o[n][h * T::W + e][i]);
+            }
+      }
+    }
+  }
+
+  // rounds r0 .. r1 - 1 of the unit
+  __device__ __forceinline__ void walk(int r0, int r1) {
+    auto first = [&](int r) {
+      const int t = r * plan.round_keys + wave_k * T::kStep;
+      return r < r1 && t < end ? t : -1;
+    };
+    int step = first(r0);
+    load_keys(step);
+    load_values(step);
+    for (int r = r0; step >= 0; ++r) {
+      const int next = first(r + 1);
+      advance(step, next);
+      step = next;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l[n] = rows_sum(l[n]);
+  }
+
+  // waves that took other positions of the same rows hand theirs to the first
+  __device__ __forceinline__ void join_waves() {
+    constexpr int kFloats = NT * (T::E * 4 + 2) * 64;
+    for (int half = key_waves / 2; half >= 1; half /= 2) {
+      float* mine = lds + (wave_r * half + wave_k % half) * kFloats;
+      __syncthreads();
+      if (wave_k >= half && wave_k < 2 * half) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float* to = mine + n * (T::E * 4 + 2) * 64;
+#pragma unroll
+          for (int e = 0; e < T::E; ++e) *reinterpret_cast<v4f*>(to + (e * 64 + lane) * 4) = o[n][e];
+          to[T::E * 256 + lane] = m[n];
+          to[T::E * 256 + 64 + lane] = l[n];
+        }
+      }
+      __syncthreads();
+      if (wave_k < half) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float* from = mine + n * (T::E * 4 + 2) * 64;
+          const float m1 = from[T::E * 256 + lane], l1 = from[T::E * 256 + 64 + lane];
+          const float most = fmaxf(m[n], m1), base = finite_base(most);
+          const float a = shift_of(m[n], base), d = shift_of(m1, base);
+          l[n] = l[n] * a + l1 * d;
+          m[n] = most;
+#pragma unroll
+          for (int e = 0; e < T::E; ++e) {
+            const v4f x = *reinterpret_cast<const v4f*>(from + (e * 64 + lane) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][e][i] = o[n][e][i] * a + x[i] * d;
+          }
+        }
+      }
+    }
+  }
+
+  // the unit's outputs, or a part's (m, l, o)
+  __device__ __forceinline__ void finish(bool complete, int64_t part) {
+    if (key_waves > 1) join_waves();
+    if (wave_k != 0) return;
+    float* scratch = static_cast<float*>(p.scratch);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + n * 16 + c;
+      if (row >= rows) continue;
+      float* to;
+      float by = 1.f;
+      if (complete) {
+        to = p.out + row_at(row);
+        by = l[n] == 0.f ? 0.f : 1.f / l[n];
+        if (kView == CacheView::kDense && p.weights && g == 0)
+          *reinterpret_cast<v2f*>(scratch + plan.stats + ((b * p.heads_kv + hkv) * rows + row) * 2) =
+              v2f{finite_base(m[n]), by};
+      } else {
+        const int64_t slot = part * plan.unit_rows + row - row0 + wave_r * NT * 16;
+        to = scratch + plan.parts_o + slot * p.dhead;
+        if (g == 0) *reinterpret_cast<v2f*>(scratch + plan.parts_ml + slot * 2) = v2f{m[n], l[n]};
+      }
+#pragma unroll
+      for (int h = 0; h < T::H; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < T::W; w += 4) {
+            const int d = (h * 16 + g * 4 + i) * T::W + w;
+            v4f x;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] = l[n] == 0.f ? 0.f : o[n][h * T::W + w + y][i] * by;
+            if (d < p.dhead) *reinterpret_cast<v4f*>(to + d) = x;
+          }
+    }
+  }
+};
+
+constexpr int waves_per_simd(int type, int dp, int nt) { return dp * nt >= 256 ? 1 : 2; }
+
+template <int kType, int DP, int NT, CacheView kView>
+__global__ __launch_bounds__(kThreads, waves_per_simd(kType, DP, NT))
+void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
+  extern __shared__ float lds[];
+  Worker<kType, DP, NT, kView> worker(p, plan, lds);
+  const int units = static_cast<int>(p.heads_kv) * plan.row_groups;
+  if (plan.whole) {
+    const int64_t b = blockIdx.x / units;
+    worker.begin(b, blockIdx.x % units);
+    worker.walk(0, uniform(rounds_of(p, plan, b)));
+    worker.finish(true, 0);
+    return;
+  }
+  const Line line = make_line(p, plan);
+  if (blockIdx.x >= line.groups) return;
+  int64_t x = line.start(blockIdx.x);
+  const int64_t x0 = x, x1 = line.start(blockIdx.x + 1);
+  // the entry that x lies in: 64 entries at a time
+  int64_t b = 0, before = 0;
+  for (;; b += 64) {
+    const int lane = threadIdx.x & 63;
+    const int64_t mine = b + lane < p.batch ? static_cast<int64_t>(rounds_of(p, plan, b + lane)) * units : 0;
+    int64_t upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(static_cast<long long>(upto), o, 64);
+      if (lane >= o) upto += y;
+    }
+    const uint64_t behind = __ballot(before + upto > x);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      before += __shfl(static_cast<long long>(upto - mine), at);
+      b += at;
+      break;
+    }
+    before += __shfl(static_cast<long long>(upto), 63);
+  }
+  b = uniform64(b);
+  before = uniform64(before);
+  while (x < x1) {
+    const int n = uniform(rounds_of(p, plan, b));
+    const int64_t within = x - before;
+    const int unit = static_cast<int>(within / n), r0 = static_cast<int>(within % n);
+    const int r1 = static_cast<int>(x1 - x < n - r0 ? r0 + (x1 - x) : n);
+    worker.begin(b, unit);
+    worker.walk(r0, r1);
+    // a part that begins the workgroup's stretch is its first, any other its last
+    worker.finish(r0 == 0 && r1 == n, blockIdx.x * 2ll + (x == x0 ? 0 : 1));
+    x += r1 - r0;
+    if (x == before + static_cast<int64_t>(n) * units) {
+      before = x;
+      ++b;
+    }
+  }
+}
+
+// The parts of a unit: which workgroups of the line hold them.
+struct Parts {
+  int64_t first, count, start;
+  Line line;
+  // slot of the i-th part
+  __device__ __forceinline__ int64_t slot(int64_t i) const {
+    return (first + i) * 2 + (line.start(first + i) >= start ? 0 : 1);
+  }
+};
+
+__device__ __forceinline__ Parts parts_of(const CacheAttnParams& p, const CachePlan& plan, int64_t b, int unit) {
+  Parts r;
+  r.line = make_line(p, plan);
+  const int64_t n = uniform(rounds_of(p, plan, b));
+  r.start = rounds_before(p, plan, b) + n * unit;
+  // workgroup w holds [w total / groups, (w + 1) total / groups): the one that holds round x is the
+  // largest w with w total / groups <= x
+  auto holder = [&](int64_t x) { return ((x + 1) * r.line.groups - 1) / r.line.total; };
+  r.first = holder(r.start);
+  r.count = holder(r.start + n - 1) - r.first + 1;
+  return r;
+}
+
+// One wave per row of a unit that has several parts: out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i
+__global__ __launch_bounds__(64) void join_kernel(CacheAttnParams p, CachePlan plan) {
+  const int lane = threadIdx.x;
+  const int group = static_cast<int>(p.heads / p.heads_kv), rows = static_cast<int>(p.tokens) * group;
+  const int row = blockIdx.x % rows;
+  const int64_t head = blockIdx.x / rows, b = head / p.heads_kv;
+  const int hkv = static_cast<int>(head % p.heads_kv);
+  const Parts parts = parts_of(p, plan, b, hkv * plan.row_groups + row / plan.unit_rows);
+  if (parts.count == 1) return;
+  const float* scratch = static_cast<const float*>(p.scratch);
+  const int local = row % plan.unit_rows;
+  const float* ml = scratch + plan.parts_ml;
+  float most = -INFINITY;
+  for (int64_t i = lane; i < parts.count; i += 64) most = fmaxf(most, ml[(parts.slot(i) * plan.unit_rows + local) * 2]);
+  most = wave_max(most);
+  const float base = finite_base(most);
+  float total = 0.f;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t i = 0; i < parts.count; ++i) {
+    const int64_t at = parts.slot(i) * plan.unit_rows + local;
+    const float weight = shift_of(ml[at * 2], base);
+    total += weight * ml[at * 2 + 1];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x * 64 + lane < p.dhead) o[x] += weight * scratch[plan.parts_o + at * p.dhead + x * 64 + lane];
+  }
+  const float by = total == 0.f ? 0.f : 1.f / total;
+  const int i = row / group;
+  float* to = p.out + ((b * p.tokens + i) * p.heads + hkv * group + row % group) * p.dhead;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (x * 64 + lane < p.dhead) to[x * 64 + lane] = total == 0.f ? 0.f : o[x] * by;
+  if (p.weights && lane == 0) {
+    float* stats = static_cast<float*>(p.scratch) + plan.stats + (head * rows + row) * 2;
+    stats[0] = base;
+    stats[1] = by;
   }
 }
 
 // weights[b, hkv, t] += sum over the group's heads of exp(s_t - m) / l
-__global__ __launch_bounds__(kThreads) void cache_weights_kernel(CacheAttnParams p) {
+__global__ __launch_bounds__(kThreads) void cache_weights_kernel(CacheAttnParams p, CachePlan plan) {
   const int64_t tiles = (p.t_max + kThreads - 1) / kThreads, unit = blockIdx.x / tiles;
-  const int64_t b = unit / p.heads_kv, hkv = unit % p.heads_kv;
   const int64_t group = p.heads / p.heads_kv;
-  int64_t len = p.lengths ? p.lengths[b] : p.length;
-  len = len < 0 ? 0 : (len > p.t_max ? p.t_max : len);
+  const int len = committed(p, unit / p.heads_kv);
   const int64_t t = blockIdx.x % tiles * kThreads + threadIdx.x;
   if (t >= len) return;
-  const float* raw = static_cast<const float*>(p.scratch);
-  const float* stats = raw + p.batch * p.heads * p.t_max;
+  const float* scores = static_cast<const float*>(p.scratch) + plan.scores + unit * group * plan.score_pitch;
+  const float* stats = static_cast<const float*>(p.scratch) + plan.stats + unit * group * 2;
   float sum = 0.f;
-  for (int64_t h = b * p.heads + hkv * group; h < b * p.heads + (hkv + 1) * group; ++h)
-    sum += expf(raw[h * p.t_max + t] - stats[2 * h]) * stats[2 * h + 1];
-  p.weights[(b * p.heads_kv + hkv) * p.t_max + t] += sum;
+  for (int64_t r = 0; r < group; ++r)
+    sum += __builtin_amdgcn_exp2f(scores[r * plan.score_pitch + t] - stats[2 * r]) * stats[2 * r + 1];
+  p.weights[unit * p.t_max + t] += sum;
 }
 
-template <typename T>
-void launch_typed(const CacheAttnParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((cache_attention_kernel<T>), dim3(static_cast<unsigned>(p.batch * p.tokens * p.heads)),
-                     dim3(kThreads), 0, stream, p);
+// ---- the host's side -------------------------------------------------------------------------
+
+int padded_head(int64_t dhead) { return dhead <= 64 ? 64 : (dhead <= 128 ? 128 : 256); }
+
+int row_tiles(const CacheAttnParams& p, int64_t rows) {
+  return rows <= 16 || p.view != CacheView::kTree || padded_head(p.dhead) == 256 ? 1 : 2;
+}
+
+CachePlan make_plan(const CacheAttnParams& p) {
+  CachePlan plan;
+  const int64_t rows = p.tokens * (p.heads / p.heads_kv);
+  const int tiles = row_tiles(p, rows);
+  plan.row_waves = rows <= 16 * tiles ? 1 : (rows <= 32 * tiles ? 2 : 4);
+  plan.unit_rows = 16 * tiles * plan.row_waves;
+  plan.row_groups = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
+  plan.round_keys = (p.kv_dtype == kF32 ? 16 : 32) * (kWaves / plan.row_waves);
+  plan.grid = 512;
+  plan.min_rounds = plan.row_waves == 1 ? 4 : 8;
+  const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
+  const int64_t units = p.batch * p.heads_kv * plan.row_groups;
+  plan.whole = walked <= plan.round_keys * plan.min_rounds || units >= 2048;
+  // scratch
+  auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
+  const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;
+  plan.parts_ml = 0;
+  plan.parts_o = up(parts * 2);
+  plan.stats = plan.parts_o + up(parts * p.dhead);
+  plan.scores = plan.stats;
+  plan.total = plan.stats;
+  plan.score_pitch = 0;
+  if (p.view == CacheView::kDense) {
+    plan.score_pitch = up(p.t_max);
+    plan.scores = plan.stats + up(p.batch * p.heads * 2);
+    plan.total = plan.scores + p.batch * p.heads * plan.score_pitch;
+  }
+  return plan;
+}
+
+template <int kType, int DP, int NT, CacheView kView>
+void launch_tiles(const CacheAttnParams& p, const CachePlan& plan, hipStream_t stream) {
+  using T = Tile<kType, DP, NT>;
+  const int64_t units = p.batch * p.heads_kv * plan.row_groups;
+  const int key_waves = kWaves / plan.row_waves;
+  const size_t lds = key_waves > 1 ? sizeof(float) * (kWaves / 2) * NT * (T::E * 4 + 2) * 64 : 0;
+  hipLaunchKernelGGL((cache_attention_kernel<kType, DP, NT, kView>),
+                     dim3(static_cast<unsigned>(plan.whole ? units : plan.grid)), dim3(kThreads), lds, stream, p, plan);
+}
+
+template <int kType, int DP>
+void launch_head(const CacheAttnParams& p, const CachePlan& plan, hipStream_t stream) {
+  if (p.view == CacheView::kDense) return launch_tiles<kType, DP, 1, CacheView::kDense>(p, plan, stream);
+  if (p.view == CacheView::kBlocks) return launch_tiles<kType, DP, 1, CacheView::kBlocks>(p, plan, stream);
+  if constexpr (DP < 256) {
+    if (plan.unit_rows / plan.row_waves == 32) return launch_tiles<kType, DP, 2, CacheView::kTree>(p, plan, stream);
+  }
+  launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
+}
+
+template <int kType>
+void launch_typed(const CacheAttnParams& p, const CachePlan& plan, hipStream_t stream) {
+  const int dp = padded_head(p.dhead);
+  if (dp == 64) launch_head<kType, 64>(p, plan, stream);
+  else if (dp == 128) launch_head<kType, 128>(p, plan, stream);
+  else launch_head<kType, 256>(p, plan, stream);
 }
 
 }  // namespace
 
 int64_t cache_attention_scratch_bytes(const CacheAttnParams& p) {
-  return p.view == CacheView::kDense ? p.batch * p.heads * (p.t_max + 2) * 4 : 0;
+  // the types differ in their rounds: as much as the larger takes
+  CacheAttnParams other = p;
+  other.kv_dtype = kF32;
+  const int64_t a = make_plan(other).total;
+  other.kv_dtype = kBF16;
+  return std::max(a, make_plan(other).total) * 4;
 }
 
 void launch_cache_attention(const CacheAttnParams& p, hipStream_t stream) {
-  if (p.kv_dtype == 0) launch_typed<float>(p, stream);
-  else if (p.kv_dtype == 4) launch_typed<__half>(p, stream);
-  else launch_typed<uint16_t>(p, stream);
+  const CachePlan plan = make_plan(p);
+  if (p.kv_dtype == kF32) launch_typed<kF32>(p, plan, stream);
+  else if (p.kv_dtype == kF16) launch_typed<kF16>(p, plan, stream);
+  else launch_typed<kBF16>(p, plan, stream);
+  if (!plan.whole)
+    hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(p.batch * p.tokens * p.heads)), dim3(64), 0, stream, p,
+                       plan);
   if (p.weights)
     hipLaunchKernelGGL(cache_weights_kernel,
                        dim3(static_cast<unsigned>((p.t_max + kThreads - 1) / kThreads * p.batch * p.heads_kv)),
-                       dim3(kThreads), 0, stream, p);
+                       dim3(kThreads), 0, stream, p, plan);
 }
 
 }  // namespace ct2x

@@ -38,8 +38,8 @@ int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 void check_cache(const char* name, int64_t batch, int64_t heads_kv, int64_t dhead, int64_t t_max) {
   CACHE_CHECK(batch >= 0 && heads_kv >= 1, "batch must be >= 0 and heads_kv >= 1");
   CACHE_CHECK(dhead >= 8 && dhead <= 256 && dhead % 8 == 0, "dhead must be a multiple of 8 in [8, 256]");
-  CACHE_CHECK(t_max >= 1 && t_max < (int64_t{1} << 31) / (dhead * 4),
-              "t_max must be >= 1 and t_max * dhead * 4 below 2^31 (one head of one entry)");
+  CACHE_CHECK(t_max >= 1 && t_max <= ((int64_t{1} << 31) - (int64_t{1} << 20)) / (dhead * 4),
+              "t_max must be >= 1 and t_max * dhead * 4 at most 2^31 - 2^20 (one head of one entry)");
   CACHE_CHECK(batch <= (int64_t{1} << 22) / heads_kv, "batch * heads_kv above 2^22");
 }
 
