@@ -37,124 +37,212 @@ __device__ __forceinline__ int64_t clamped_length(const int32_t* lengths, int64_
   return n < 0 ? 0 : (n > t_max ? t_max : n);
 }
 
+template <typename K>
+__device__ __forceinline__ K wave_and(K x) {
+  for (int o = 32; o > 0; o >>= 1) x &= static_cast<K>(__shfl_xor(static_cast<unsigned long long>(x), o, 64));
+  return x;
+}
+
 // The `want` (>= 1, <= n) best of key(0 .. n): *threshold = the smallest key taken, returns how many
-// of the keys equal to it are taken. All threads of the workgroup call.
+// of the keys equal to it are taken. All threads of the workgroup call. Bits that all keys share are
+// skipped (a first pass finds them: scores of one layer have their exponent in common, and every key
+// would meet in one bin), and the search ends with the byte whose bin is taken whole.
 template <typename K, typename F>
-__device__ int64_t select_threshold(F key, int64_t n, int64_t want, K* threshold) {
+__device__ int select_threshold(F key, int n, int want, K* threshold) {
   __shared__ uint32_t histogram[256];
-  __shared__ uint32_t digit_s;
-  __shared__ uint32_t above_s;
-  K prefix = 0, known = 0;
-  for (int shift = sizeof(K) * 8 - 8; shift >= 0; shift -= 8) {
+  __shared__ K both_s[kSelectThreads / 64], none_s[kSelectThreads / 64];
+  __shared__ uint32_t digit_s, above_s, count_s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  K both = ~static_cast<K>(0), none = both;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += kSelectThreads) {
+    const K x = key(i);
+    both &= x;
+    none &= ~x;
+  }
+  both = wave_and(both);
+  none = wave_and(none);
+  if (lane == 0) {
+    both_s[wave] = both;
+    none_s[wave] = none;
+  }
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) {
+    both &= both_s[w];
+    none &= none_s[w];
+  }
+  const K differ = ~(both | none);
+  if (differ == 0) {
+    *threshold = both;
+    return want;
+  }
+  int upto = 64 - __clzll(static_cast<unsigned long long>(differ));  // bits below `upto` are searched
+  K known = upto >= static_cast<int>(sizeof(K)) * 8 ? 0 : ~static_cast<K>(0) << upto;
+  K prefix = both & known;
+  while (upto > 0) {
+    const int bits = upto < 8 ? upto : 8, shift = upto - bits;
     __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) histogram[i] = 0;
+    if (threadIdx.x < 256) histogram[threadIdx.x] = 0;
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kSelectThreads) {
       const K x = key(i);
-      if ((x & known) == prefix) atomicAdd(&histogram[(x >> shift) & 255], 1u);
+      if ((x & known) == prefix) atomicAdd(&histogram[(x >> shift) & ((1u << bits) - 1)], 1u);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int64_t above = 0;
-      int digit = 255;
-      while (above + histogram[digit] < want) above += histogram[digit--];
-      digit_s = digit;
-      above_s = static_cast<uint32_t>(above);
+    if (wave == 0) {  // lane 0 has the four highest bins
+      uint32_t bin[4], sum = 0;
+      for (int i = 0; i < 4; ++i) sum += bin[i] = histogram[255 - 4 * lane - i];
+      uint32_t upto_lane = sum;
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(upto_lane, o, 64);
+        if (lane >= o) upto_lane += y;
+      }
+      const uint64_t reached = __ballot(upto_lane >= static_cast<uint32_t>(want));
+      if (lane == __builtin_ctzll(reached)) {
+        uint32_t above = upto_lane - sum;
+        int i = 0;
+        while (i < 3 && above + bin[i] < static_cast<uint32_t>(want)) above += bin[i++];
+        digit_s = 255 - 4 * lane - i;
+        above_s = above;
+        count_s = bin[i];
+      }
     }
     __syncthreads();
     want -= above_s;
     prefix |= static_cast<K>(digit_s) << shift;
-    known |= static_cast<K>(255) << shift;
+    known |= static_cast<K>((1u << bits) - 1) << shift;
+    upto = shift;
+    if (count_s == static_cast<uint32_t>(want)) {
+      // everything with this prefix is taken: nothing below it is, whatever its lower bits. (As a
+      // threshold the prefix itself: it may be no key, then none is equal to it and all are above.)
+      break;
+    }
   }
   *threshold = prefix;
   return want;
 }
 
 // emit(slot, i) for the i of 0 .. n with key(i) > threshold or among the first `ties` equal to it,
-// slots 0, 1, .. in order of i. Returns how many. All threads of the workgroup call.
+// slots 0, 1, .. in order of i. Returns how many. All threads of the workgroup call. A wave takes a
+// stretch of positions: it counts, the waves add up, it emits.
 template <typename K, typename F, typename G>
-__device__ int64_t emit_selected(F key, int64_t n, K threshold, int64_t ties, G emit) {
-  __shared__ uint32_t taken_s[kSelectThreads / 64], equal_s[kSelectThreads / 64];
+__device__ int emit_selected(F key, int n, K threshold, int ties, G emit) {
+  __shared__ int above_w[kSelectThreads / 64], equal_w[kSelectThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  int64_t slot = 0, equal = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += blockDim.x) {
-    const int64_t i = i0 + threadIdx.x;
-    const K x = i < n ? key(i) : 0;
-    const bool same = i < n && x == threshold;
-    const uint64_t same_bits = __ballot(same), below = (1ull << lane) - 1;
-    if (lane == 0) equal_s[wave] = __popcll(same_bits);
-    __syncthreads();
-    int64_t rank = equal, all = equal;
-    for (int w = 0; w < waves; ++w) {
-      if (w < wave) rank += equal_s[w];
-      all += equal_s[w];
+  const int stretch = ((n + waves - 1) / waves + 63) / 64 * 64;
+  const int from = wave * stretch, to = from + stretch < n ? from + stretch : n;
+  int above = 0, equal = 0;
+  constexpr int kAhead = 4;  // keys requested together
+  for (int i0 = from; i0 < to; i0 += 64 * kAhead) {
+    K x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * 64 + lane < to ? key(i0 + u * 64 + lane) : 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool there = i0 + u * 64 + lane < to;
+      above += __popcll(__ballot(there && x[u] > threshold));
+      equal += __popcll(__ballot(there && x[u] == threshold));
     }
-    rank += __popcll(same_bits & below);
-    const bool take = i < n && (x > threshold || (same && rank < ties));
-    const uint64_t take_bits = __ballot(take);
-    if (lane == 0) taken_s[wave] = __popcll(take_bits);
-    __syncthreads();
-    int64_t at = slot, next = slot;
-    for (int w = 0; w < waves; ++w) {
-      if (w < wave) at += taken_s[w];
-      next += taken_s[w];
-    }
-    if (take) emit(at + __popcll(take_bits & below), i);
-    slot = next;
-    equal = all;
-    __syncthreads();
   }
-  return slot;
+  if (lane == 0) {
+    above_w[wave] = above;
+    equal_w[wave] = equal;
+  }
+  __syncthreads();
+  int slot = 0, rank = 0, all = 0, all_equal = 0;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wave) {
+      slot += above_w[w];
+      rank += equal_w[w];
+    }
+    all += above_w[w];
+    all_equal += equal_w[w];
+  }
+  slot += rank < ties ? rank : ties;
+  const uint64_t below = (1ull << lane) - 1;
+  for (int i0 = from; i0 < to; i0 += 64 * kAhead) {
+    K x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * 64 + lane < to ? key(i0 + u * 64 + lane) : 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * 64 + lane;
+      const bool same = i < to && x[u] == threshold;
+      const uint64_t same_bits = __ballot(same);
+      const bool take = i < to && (x[u] > threshold || (same && rank + __popcll(same_bits & below) < ties));
+      const uint64_t bits = __ballot(take);
+      if (take) emit(slot + __popcll(bits & below), i);
+      slot += __popcll(bits);
+      rank += __popcll(same_bits);
+    }
+  }
+  return all + (all_equal < ties ? all_equal : ties);
 }
 
 // positions[b, hkv, :]: what stays, ascending, -1 behind the last
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvictParams p) {
   const int64_t row = blockIdx.x, b = row / p.heads_kv;
-  const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
+  const int n = static_cast<int>(clamped_length(p.lengths, p.length, b, p.t_max));
+  const int budget = static_cast<int>(p.budget), recent = static_cast<int>(p.recent);
   const float* w = p.weights + row * p.t_max;
   int32_t* positions = p.positions + row * p.budget;
-  const int64_t kept = n < p.budget ? n : p.budget;
-  int64_t slot = 0, old = 0;
-  if (n > p.budget && p.budget > p.recent) {
-    old = n - p.recent;
-    auto key = [&](int64_t i) { return order_key(w[i]); };
+  const int kept = n < budget ? n : budget;
+  int slot = 0;
+  if (n > budget && budget > recent) {
+    const int old = n - recent;
+    auto key = [&](int i) { return order_key(w[i]); };
     uint32_t threshold;
-    const int64_t ties = select_threshold<uint32_t>(key, old, p.budget - p.recent, &threshold);
-    slot = emit_selected<uint32_t>(key, old, threshold, ties,
-                                   [&](int64_t at, int64_t i) { positions[at] = static_cast<int32_t>(i); });
+    const int ties = select_threshold<uint32_t>(key, old, budget - recent, &threshold);
+    slot = emit_selected<uint32_t>(key, old, threshold, ties, [&](int at, int i) { positions[at] = i; });
   }
-  for (int64_t i = slot + threadIdx.x; i < p.budget; i += blockDim.x)
-    positions[i] = i < kept ? static_cast<int32_t>(n - kept + i) : -1;
+  for (int i = slot + threadIdx.x; i < budget; i += blockDim.x) positions[i] = i < kept ? n - kept + i : -1;
 }
 
-// One workgroup moves 256 bytes of every kept row of a (entry, head)'s keys or values, in steps
-// that are read before they are written: a row moves to the front only, so that a step never
-// overwrites what a later one reads and the output may be the input.
-__global__ __launch_bounds__(kThreads) void evict_move_kernel(CacheEvictParams p, int row_bytes, int slices) {
-  constexpr int kRows = kThreads / 16;
-  const int64_t row = blockIdx.x / (2 * slices);
-  const int slice = blockIdx.x % slices, value = blockIdx.x / slices % 2;
-  const int64_t b = row / p.heads_kv;
+// A workgroup moves one cache line (128 bytes) of the kept rows of a (entry, head)'s keys or values,
+// kMoveSteps rows per thread between two barriers. Rows only ever move to the front, so that the rows
+// of a step are read before any later step's place is written: one workgroup that takes all steps in
+// turn may write where it reads. Apart, `chunks` workgroups take the steps.
+constexpr int kMoveThreads = 512, kMoveSteps = 4;
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(CacheEvictParams p, int row_bytes, int slices,
+                                                                  int chunks) {
+  constexpr int kRows = kMoveThreads / 8;
+  const int chunk = blockIdx.x % chunks, part = blockIdx.x / chunks % (2 * slices);
+  const int64_t row = blockIdx.x / chunks / (2 * slices), b = row / p.heads_kv;
+  const int slice = part >> 1, value = part & 1;
   const int32_t* positions = p.positions + row * p.budget;
   const char* from = static_cast<const char*>(value ? p.v : p.k) + row * p.t_max * row_bytes;
   char* to = static_cast<char*>(value ? p.v_out : p.k_out) + row * p.t_max_out * row_bytes;
   const float* w = p.weights + row * p.t_max;
   float* w_out = p.weights_out + row * p.t_max_out;
-  const int at = slice * 256 + (threadIdx.x & 15) * 16;
-  for (int64_t j0 = 0; j0 < p.budget; j0 += kRows) {
-    const int64_t j = j0 + threadIdx.x / 16;
-    const int32_t t = j < p.budget ? positions[j] : -1;
-    const bool moves = t >= 0 && at < row_bytes;
-    const bool first = t >= 0 && (threadIdx.x & 15) == 0 && blockIdx.x % (2 * slices) == 0;
-    int4 data = {0, 0, 0, 0};
-    float weight = 0.f;
-    if (moves) data = *reinterpret_cast<const int4*>(from + t * static_cast<int64_t>(row_bytes) + at);
-    if (first) weight = w[t];
+  const int at = slice * 128 + (threadIdx.x & 7) * 16, budget = static_cast<int>(p.budget);
+  const bool weighs = part == 0 && (threadIdx.x & 7) == 0;
+  for (int j0 = chunk * kRows * kMoveSteps; j0 < budget; j0 += chunks * kRows * kMoveSteps) {
+    int4 data[kMoveSteps];
+    float weight[kMoveSteps];
+    int t[kMoveSteps];
+#pragma unroll
+    for (int i = 0; i < kMoveSteps; ++i) {
+      const int j = j0 + i * kRows + (threadIdx.x >> 3);
+      t[i] = j < budget ? positions[j] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kMoveSteps; ++i) {
+      data[i] = int4{0, 0, 0, 0};
+      weight[i] = 0.f;
+      if (t[i] >= 0 && at < row_bytes)
+        data[i] = *reinterpret_cast<const int4*>(from + t[i] * static_cast<int64_t>(row_bytes) + at);
+      if (t[i] >= 0 && weighs) weight[i] = w[t[i]];
+    }
     __syncthreads();
-    if (moves) *reinterpret_cast<int4*>(to + j * row_bytes + at) = data;
-    if (first) w_out[j] = weight;
+#pragma unroll
+    for (int i = 0; i < kMoveSteps; ++i) {
+      const int64_t j = j0 + i * kRows + (threadIdx.x >> 3);
+      if (t[i] >= 0 && at < row_bytes) *reinterpret_cast<int4*>(to + j * row_bytes + at) = data[i];
+      if (t[i] >= 0 && weighs) w_out[j] = weight[i];
+    }
   }
-  if (blockIdx.x % (2 * slices * p.heads_kv) == 0 && threadIdx.x == 0) {
+  if (blockIdx.x % (2 * slices * chunks * p.heads_kv) == 0 && threadIdx.x == 0) {
     const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
     p.lengths_out[b] = static_cast<int32_t>(n < p.budget ? n : p.budget);
   }
@@ -169,97 +257,197 @@ __device__ __forceinline__ float load_float(__half x) { return __half2float(x); 
 template <>
 __device__ __forceinline__ float load_float(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
 
-// One thread per channel of a (entry, head, block). NaN keys make NaN bounds.
+// the way back of a value that came from T
 template <typename T>
-__global__ __launch_bounds__(kThreads) void block_bounds_kernel(CacheBoundsParams p, int64_t blocks) {
-  const int64_t j = blockIdx.x % blocks, row = blockIdx.x / blocks, b = row / p.heads_kv;
-  const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
-  int64_t first = p.first ? p.first[b] : 0;
-  first = first < 0 ? 0 : first;
-  if (j < first / p.block || j * p.block >= n) return;
-  const int64_t end = (j + 1) * p.block < n ? (j + 1) * p.block : n;
-  const T* k = static_cast<const T*>(p.k) + row * p.t_max * p.dhead;
-  T* out = static_cast<T*>(p.bounds) + (row * blocks + j) * 2 * p.dhead;
-  for (int64_t d = threadIdx.x; d < p.dhead; d += kThreads) {
-    T low = k[j * p.block * p.dhead + d], high = low;
-    for (int64_t t = j * p.block + 1; t < end; ++t) {
-      const T x = k[t * p.dhead + d];
-      const float f = load_float(x);
-      if (!(f >= load_float(low)) && load_float(low) == load_float(low)) low = x;
-      if (!(f <= load_float(high)) && load_float(high) == load_float(high)) high = x;
+__device__ __forceinline__ T store_float(float x);
+template <>
+__device__ __forceinline__ float store_float(float x) { return x; }
+template <>
+__device__ __forceinline__ __half store_float(float x) { return __float2half(x); }
+template <>
+__device__ __forceinline__ uint16_t store_float(float x) { return static_cast<uint16_t>(__float_as_uint(x) >> 16); }
+
+// 16 bytes of a row as floats
+template <typename T>
+__device__ __forceinline__ void unpack(const int4& x, float (&y)[16 / sizeof(T)]) {
+  const T* t = reinterpret_cast<const T*>(&x);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) y[i] = load_float(t[i]);
+}
+
+// A wave per (entry, head, block): 16 bytes of a row per lane, lanes of the same channels joined by
+// lane exchanges. Rows behind the end repeat the last one, which changes no minimum. minimum /
+// maximum hand on a NaN, and every bound is a key's value, so the way back to 16 bits is exact.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void block_bounds_kernel(CacheBoundsParams p, int64_t blocks, int walkers,
+                                                                int lanes) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t row = blockIdx.x / walkers, b = row / p.heads_kv;
+  const int n = static_cast<int>(clamped_length(p.lengths, p.length, b, p.t_max));
+  const int block = static_cast<int>(p.block);
+  int first = p.first ? p.first[b] : 0;
+  first = first < 0 ? 0 : first / block;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int channel = (lane & (lanes - 1)) * V, at = lane / lanes, step = 64 / lanes;
+  const bool there = channel < p.dhead;
+  const T* k = static_cast<const T*>(p.k) + row * p.t_max * p.dhead + (there ? channel : 0);
+  for (int64_t j = first + blockIdx.x % walkers * (kThreads / 64) + wave; j * block < n; j += walkers * (kThreads / 64)) {
+    const int start = static_cast<int>(j) * block, last = (start + block < n ? start + block : n) - 1;
+    float low[V], high[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      low[i] = INFINITY;
+      high[i] = -INFINITY;
     }
-    out[d] = low;
-    out[p.dhead + d] = high;
+    for (int t = start + at; t <= last + at; t += 8 * step) {
+      int4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t from = t + u * step < last ? t + u * step : last;
+        x[u] = *reinterpret_cast<const int4*>(k + from * p.dhead);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float y[V];
+        unpack<T>(x[u], y);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          low[i] = __builtin_elementwise_minimum(low[i], y[i]);
+          high[i] = __builtin_elementwise_maximum(high[i], y[i]);
+        }
+      }
+    }
+    for (int o = lanes; o < 64; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        low[i] = __builtin_elementwise_minimum(low[i], __shfl_xor(low[i], o, 64));
+        high[i] = __builtin_elementwise_maximum(high[i], __shfl_xor(high[i], o, 64));
+      }
+    if (lane < lanes && there) {
+      T out[2][V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        out[0][i] = store_float<T>(low[i]);
+        out[1][i] = store_float<T>(high[i]);
+      }
+      T* to = static_cast<T*>(p.bounds) + (row * blocks + j) * 2 * p.dhead + channel;
+      *reinterpret_cast<int4*>(to) = *reinterpret_cast<const int4*>(out[0]);
+      *reinterpret_cast<int4*>(to + p.dhead) = *reinterpret_cast<const int4*>(out[1]);
+    }
   }
 }
 
-// scores[b, hkv, j] = max over the group's heads of sum_d max(q_d min_d, q_d max_d), float64: a
-// choice between blocks must not depend on how the sum was ordered.
+// scores[b, hkv, j] = max over the group's heads of sum_d (q_d >= 0 ? q_d max_d : q_d min_d), NaN where
+// a bound is; float64, since a choice between blocks must not depend on how the sum was ordered. Eight
+// lanes per block, each with every eighth 16 bytes of its channels; the heads' queries wait in LDS as
+// float64. Bound by the reads of the bounds.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParams p, int64_t blocks) {
-  const int64_t tiles = (blocks + kThreads - 1) / kThreads, row = blockIdx.x / tiles;
-  const int64_t b = row / p.heads_kv, hkv = row % p.heads_kv, group = p.heads / p.heads_kv;
+__global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParams p, int64_t blocks, int walkers) {
+  constexpr int V = 16 / sizeof(T), kHeads = 4;  // heads at a time
+  __shared__ double q_s[kHeads][256];
+  const int64_t row = blockIdx.x / walkers;
+  const int64_t b = row / p.heads_kv, hkv = row % p.heads_kv;
+  const int group = static_cast<int>(p.heads / p.heads_kv), dhead = static_cast<int>(p.dhead);
   const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
-  const int64_t j = blockIdx.x % tiles * static_cast<int64_t>(kThreads) + threadIdx.x;
-  if (j * p.block >= n) return;
-  const T* low = static_cast<const T*>(p.bounds) + (row * blocks + j) * 2 * p.dhead;
-  double best = 0.;
-  for (int64_t g = 0; g < group; ++g) {
-    const float* q = p.q + (b * p.heads + hkv * group + g) * p.dhead;
-    double sum = 0.;
-    for (int64_t d = 0; d < p.dhead; ++d) {
-      const double x = q[d], a = x * load_float(low[d]), c = x * load_float(low[p.dhead + d]);
-      sum += a != a || a > c ? a : c;
+  const int count = static_cast<int>((n + p.block - 1) / p.block);
+  const int per = (count + walkers * 32 - 1) / (walkers * 32) * 32, from = static_cast<int>(blockIdx.x % walkers) * per;
+  const int to = from + per < count ? from + per : count;
+  if (from >= to || count <= p.top) return;  // (all blocks are taken: no scores are looked at)
+  const int part = threadIdx.x & 7;
+  const T* bounds = static_cast<const T*>(p.bounds) + row * blocks * 2 * dhead;
+  for (int h0 = 0; h0 < group; h0 += kHeads) {
+    const int heads = group - h0 < kHeads ? group - h0 : kHeads;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kHeads * dhead; i += kThreads)
+      q_s[i / dhead][i % dhead] =
+          i / dhead < heads ? p.q[(b * p.heads + hkv * group + h0) * dhead + i] : 0.;
+    __syncthreads();
+    for (int j0 = from; j0 < to; j0 += kThreads / 8) {
+      const int j = j0 + (threadIdx.x >> 3);
+      const T* low = bounds + static_cast<int64_t>(j < to ? j : to - 1) * 2 * dhead;
+      double sum[kHeads] = {0., 0., 0., 0.};
+      bool fine = true;
+      for (int d = part * V; d < dhead; d += 8 * V) {
+        float x[V], y[V];
+        unpack<T>(*reinterpret_cast<const int4*>(low + d), x);
+        unpack<T>(*reinterpret_cast<const int4*>(low + dhead + d), y);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          fine &= x[i] == x[i] && y[i] == y[i];
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) {
+            const double q = q_s[h][d + i];
+            sum[h] = fma(q, static_cast<double>(q >= 0. ? y[i] : x[i]), sum[h]);
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
+        for (int o = 1; o < 8; o <<= 1) sum[h] += __shfl_xor(sum[h], o, 64);
+      for (int o = 1; o < 8; o <<= 1) fine &= __shfl_xor(static_cast<int>(fine), o, 64) != 0;
+      if (part == 0 && j < to) {
+        double best = h0 ? p.scores[row * blocks + j] : sum[0];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+          if (h < heads && (sum[h] > best || sum[h] != sum[h])) best = sum[h];
+        p.scores[row * blocks + j] = fine ? best : __builtin_nan("");
+      }
     }
-    if (g == 0 || sum > best || sum != sum) best = sum;
-    if (best != best) break;
   }
-  p.scores[row * blocks + j] = best;
 }
 
 __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(CacheSelectParams p, int64_t blocks) {
   const int64_t row = blockIdx.x, b = row / p.heads_kv;
   const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
-  const int64_t count = (n + p.block - 1) / p.block;
+  const int count = static_cast<int>((n + p.block - 1) / p.block), top = static_cast<int>(p.top);
   const double* scores = p.scores + row * blocks;
   int32_t* selected = p.selected + row * p.top;
-  int64_t taken = count;
-  if (count > p.top) {
-    auto key = [&](int64_t j) {
-      return j < p.sink || j >= count - p.local ? ~0ull : order_key(scores[j]);
-    };
+  if (count > top) {
+    auto key = [&](int j) { return j < p.sink || j >= count - p.local ? ~0ull : order_key(scores[j]); };
     uint64_t threshold;
-    const int64_t ties = select_threshold<uint64_t>(key, count, p.top, &threshold);
-    emit_selected<uint64_t>(key, count, threshold, ties,
-                            [&](int64_t at, int64_t j) { selected[at] = static_cast<int32_t>(j); });
-    taken = p.top;
+    const int ties = select_threshold<uint64_t>(key, count, top, &threshold);
+    emit_selected<uint64_t>(key, count, threshold, ties, [&](int at, int j) { selected[at] = j; });
   } else {
-    for (int64_t j = threadIdx.x; j < count; j += blockDim.x) selected[j] = static_cast<int32_t>(j);
+    for (int j = threadIdx.x; j < top; j += blockDim.x) selected[j] = j < count ? j : -1;
   }
-  for (int64_t j = taken + threadIdx.x; j < p.top; j += blockDim.x) selected[j] = -1;
+}
+
+// Workgroups per (entry, head): enough for eight on every CU, at most one for `pieces` each.
+int walkers_for(int64_t rows, int64_t pieces) {
+  const int64_t fill = (2048 + rows - 1) / rows;
+  return static_cast<int>(fill < pieces ? fill : pieces);
 }
 
 template <typename T>
 void bounds_typed(const CacheBoundsParams& p, int64_t blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((block_bounds_kernel<T>), dim3(static_cast<unsigned>(p.batch * p.heads_kv * blocks)),
-                     dim3(kThreads), 0, stream, p, blocks);
+  const int64_t rows = p.batch * p.heads_kv;
+  const int walkers = walkers_for(rows, (blocks + kThreads / 64 - 1) / (kThreads / 64));
+  int lanes = 1;
+  while (lanes * 16 < static_cast<int>(p.dhead * sizeof(T))) lanes *= 2;
+  hipLaunchKernelGGL((block_bounds_kernel<T>), dim3(static_cast<unsigned>(rows * walkers)), dim3(kThreads), 0, stream,
+                     p, blocks, walkers, lanes);
 }
 
 template <typename T>
 void scores_typed(const CacheSelectParams& p, int64_t blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((block_scores_kernel<T>),
-                     dim3(static_cast<unsigned>((blocks + kThreads - 1) / kThreads * p.batch * p.heads_kv)),
-                     dim3(kThreads), 0, stream, p, blocks);
+  const int64_t rows = p.batch * p.heads_kv;
+  const int walkers = walkers_for(rows, (blocks + kThreads / 8 - 1) / (kThreads / 8));
+  hipLaunchKernelGGL((block_scores_kernel<T>), dim3(static_cast<unsigned>(rows * walkers)), dim3(kThreads), 0, stream,
+                     p, blocks, walkers);
 }
 
 }  // namespace
 
 void launch_cache_evict(const CacheEvictParams& p, hipStream_t stream) {
   const int row_bytes = static_cast<int>(p.dhead) * (p.kv_dtype == 0 ? 4 : 2);
-  const int slices = (row_bytes + 255) / 256;
-  const unsigned rows = static_cast<unsigned>(p.batch * p.heads_kv);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(rows), dim3(kSelectThreads), 0, stream, p);
-  hipLaunchKernelGGL(evict_move_kernel, dim3(rows * 2 * slices), dim3(kThreads), 0, stream, p, row_bytes, slices);
+  const int slices = (row_bytes + 127) / 128;
+  const int64_t rows = p.batch * p.heads_kv;
+  const int64_t steps = (p.budget + kMoveThreads / 8 * kMoveSteps - 1) / (kMoveThreads / 8 * kMoveSteps);
+  // in place the steps have an order
+  const int chunks = p.k == p.k_out || p.v == p.v_out || p.weights == p.weights_out ? 1 : walkers_for(rows * 2 * slices, steps);
+  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, stream, p);
+  hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(rows * 2 * slices * chunks)), dim3(kMoveThreads), 0,
+                     stream, p, row_bytes, slices, chunks);
 }
 
 void launch_cache_block_bounds(const CacheBoundsParams& p, hipStream_t stream) {

@@ -598,8 +598,9 @@ int ct2x_cache_block_bounds(const void* d_k_cache, int kv_dtype, const int32_t* 
                             int64_t dhead, int64_t t_max, int64_t block, void* d_bounds, void* stream);
 
 /* The attention of one decode step over selected blocks of the cache: d_q, d_out [batch, heads,
- * dhead]. A block's score is max over the heads of the group of sum_d max(q_d min_d, q_d max_d) with
- * d_bounds of ct2x_cache_block_bounds - no key of the block scores higher -, summed in float64. The
+ * dhead]. A block's score is max over the heads of the group of sum_d (q_d >= 0 ? q_d max_d : q_d
+ * min_d) with d_bounds of ct2x_cache_block_bounds - no key of the block scores higher -, summed in
+ * float64; NaN where a bound is NaN. The
  * first `sink` and the last `local` blocks of the entry are always taken, then the best of the others
  * up to `top` in all (equal scores: the earlier block; NaN counts as the largest); entries of at most
  * `top` blocks read them all. The heads of a group share the choice. d_selected [batch, heads_kv,
