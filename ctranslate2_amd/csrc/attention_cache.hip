@@ -24,7 +24,8 @@
 // Work is cut evenly whatever the lengths: the rounds (kStep positions per wave that shares a row
 // group) of all (entry, head, row group) units form one line, workgroup w of G takes the w-th G-th of
 // it. A unit that lies within one workgroup is finished there; the others leave (m, l, o) per part
-// and join_kernel adds them. A workgroup leaves at most two such parts (its first and its last unit).
+// and finish_kernel adds them. A workgroup leaves at most two such parts (its first and its last
+// unit); the one that begins a unit writes down where its parts are.
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
@@ -66,7 +67,9 @@ struct CachePlan {
   bool whole;       // one workgroup per unit
   int64_t score_pitch;  // accumulate: floats between the score rows
   // scratch, in floats
-  int64_t parts_ml, parts_o, stats, scores, total;
+  int64_t records, parts_ml, parts_o, stats, scores, total;
+  int join_groups;  // workgroups of finish_kernel that join parts
+  int weight_tiles; // and those per (entry, head) that add up the weights
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -96,11 +99,21 @@ __device__ __forceinline__ int rounds_of(const CacheAttnParams& p, const CachePl
   return n < 1 ? 1 : n;
 }
 
-// The line of all rounds: its length and how many workgroups share it.
+// a / b of what fits 32 bits in all but the largest calls
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if ((a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The line of all rounds and how many workgroups share it: the first `longer` take `each` + 1 rounds.
 struct Line {
-  int64_t total;
-  int64_t groups;
-  __device__ __forceinline__ int64_t start(int64_t w) const { return w * total / groups; }
+  int64_t total, groups, each, longer;
+  __device__ __forceinline__ int64_t start(int64_t w) const { return w * each + (w < longer ? w : longer); }
+  // the workgroup that holds round x
+  __device__ __forceinline__ int64_t holder(int64_t x) const {
+    const int64_t ahead = longer * (each + 1);
+    return x < ahead ? divide(x, each + 1) : longer + divide(x - ahead, each);
+  }
 };
 
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
@@ -118,8 +131,10 @@ __device__ __forceinline__ int64_t rounds_before(const CacheAttnParams& p, const
 __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CachePlan& plan) {
   Line line;
   line.total = rounds_before(p, plan, p.batch);
-  const int64_t groups = line.total / plan.min_rounds;
+  const int64_t groups = divide(line.total, plan.min_rounds);
   line.groups = groups < 1 ? 1 : (groups > plan.grid ? plan.grid : groups);
+  line.each = divide(line.total, line.groups);
+  line.longer = line.total - line.each * line.groups;
   return line;
 }
 
@@ -685,12 +700,17 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
   while (x < x1) {
     const int n = uniform(rounds_of(p, plan, b));
     const int64_t within = x - before;
-    const int unit = static_cast<int>(within / n), r0 = static_cast<int>(within % n);
+    const int unit = static_cast<int>(divide(within, n)), r0 = static_cast<int>(within - static_cast<int64_t>(unit) * n);
     const int r1 = static_cast<int>(x1 - x < n - r0 ? r0 + (x1 - x) : n);
     worker.begin(b, unit);
     worker.walk(r0, r1);
     // a part that begins the workgroup's stretch is its first, any other its last
-    worker.finish(r0 == 0 && r1 == n, blockIdx.x * 2ll + (x == x0 ? 0 : 1));
+    const int slot = blockIdx.x * 2 + (x == x0 ? 0 : 1);
+    if (r0 == 0 && threadIdx.x == 0) {
+      const int count = static_cast<int>(line.holder(x + n - 1)) - static_cast<int>(blockIdx.x) + 1;
+      reinterpret_cast<int2*>(static_cast<float*>(p.scratch) + plan.records)[b * units + unit] = int2{slot, count};
+    }
+    worker.finish(r0 == 0 && r1 == n, slot);
     x += r1 - r0;
     if (x == before + static_cast<int64_t>(n) * units) {
       before = x;
@@ -699,81 +719,126 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
   }
 }
 
-// The parts of a unit: which workgroups of the line hold them.
+// Where the parts of a unit are: the first in its slot, the others in the first slots of the
+// workgroups that follow.
 struct Parts {
-  int64_t first, count, start;
-  Line line;
-  // slot of the i-th part
-  __device__ __forceinline__ int64_t slot(int64_t i) const {
-    return (first + i) * 2 + (line.start(first + i) >= start ? 0 : 1);
+  int first, count;
+  __device__ __forceinline__ Parts(const CacheAttnParams& p, const CachePlan& plan, int64_t unit) {
+    const int2 record =
+        reinterpret_cast<const int2*>(static_cast<const float*>(p.scratch) + plan.records)[unit];
+    first = record.x;
+    count = record.y;
+  }
+  __device__ __forceinline__ int64_t row(const CachePlan& plan, int i, int local) const {
+    return static_cast<int64_t>(i == 0 ? first : ((first >> 1) + i) * 2) * plan.unit_rows + local;
   }
 };
 
-__device__ __forceinline__ Parts parts_of(const CacheAttnParams& p, const CachePlan& plan, int64_t b, int unit) {
-  Parts r;
-  r.line = make_line(p, plan);
-  const int64_t n = uniform(rounds_of(p, plan, b));
-  r.start = rounds_before(p, plan, b) + n * unit;
-  // workgroup w holds [w total / groups, (w + 1) total / groups): the one that holds round x is the
-  // largest w with w total / groups <= x
-  auto holder = [&](int64_t x) { return ((x + 1) * r.line.groups - 1) / r.line.total; };
-  r.first = holder(r.start);
-  r.count = holder(r.start + n - 1) - r.first + 1;
-  return r;
-}
-
-// One wave per row of a unit that has several parts: out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i
-__global__ __launch_bounds__(64) void join_kernel(CacheAttnParams p, CachePlan plan) {
-  const int lane = threadIdx.x;
+// One wave per row of a unit with several parts: out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i
+__device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
+  constexpr int kAhead = 4;  // parts requested together
+  const int lane = threadIdx.x & 63;
   const int group = static_cast<int>(p.heads / p.heads_kv), rows = static_cast<int>(p.tokens) * group;
-  const int row = blockIdx.x % rows;
-  const int64_t head = blockIdx.x / rows, b = head / p.heads_kv;
-  const int hkv = static_cast<int>(head % p.heads_kv);
-  const Parts parts = parts_of(p, plan, b, hkv * plan.row_groups + row / plan.unit_rows);
+  const int64_t at = blockIdx.x * static_cast<int64_t>(kWaves) + uniform(threadIdx.x >> 6);
+  const int64_t unit = at / plan.unit_rows, head = unit / plan.row_groups;
+  if (head >= p.batch * p.heads_kv) return;
+  const int local = static_cast<int>(at - unit * plan.unit_rows);
+  const int row = static_cast<int>(unit - head * plan.row_groups) * plan.unit_rows + local;
+  if (row >= rows) return;
+  const Parts parts(p, plan, unit);
   if (parts.count == 1) return;
   const float* scratch = static_cast<const float*>(p.scratch);
-  const int local = row % plan.unit_rows;
-  const float* ml = scratch + plan.parts_ml;
+  const v2f* ml = reinterpret_cast<const v2f*>(scratch + plan.parts_ml);
   float most = -INFINITY;
-  for (int64_t i = lane; i < parts.count; i += 64) most = fmaxf(most, ml[(parts.slot(i) * plan.unit_rows + local) * 2]);
+  for (int i = lane; i < parts.count; i += 64) most = fmaxf(most, ml[parts.row(plan, i, local)][0]);
   most = wave_max(most);
   const float base = finite_base(most);
   float total = 0.f;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t i = 0; i < parts.count; ++i) {
-    const int64_t at = parts.slot(i) * plan.unit_rows + local;
-    const float weight = shift_of(ml[at * 2], base);
-    total += weight * ml[at * 2 + 1];
+  for (int i0 = 0; i0 < parts.count; i0 += kAhead) {
+    v2f part[kAhead];
+    float x[kAhead][4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (x * 64 + lane < p.dhead) o[x] += weight * scratch[plan.parts_o + at * p.dhead + x * 64 + lane];
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t from = parts.row(plan, i0 + u < parts.count ? i0 + u : 0, local);
+      part[u] = ml[from];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        x[u][c] = c * 64 + lane < p.dhead ? scratch[plan.parts_o + from * p.dhead + c * 64 + lane] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u >= parts.count) break;
+      const float weight = shift_of(part[u][0], base);
+      total += weight * part[u][1];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] += weight * x[u][c];
+    }
   }
   const float by = total == 0.f ? 0.f : 1.f / total;
+  const int64_t b = head / p.heads_kv, hkv = head - b * p.heads_kv;
   const int i = row / group;
-  float* to = p.out + ((b * p.tokens + i) * p.heads + hkv * group + row % group) * p.dhead;
+  float* to = p.out + ((b * p.tokens + i) * p.heads + hkv * group + row - i * group) * p.dhead;
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
-    if (x * 64 + lane < p.dhead) to[x * 64 + lane] = total == 0.f ? 0.f : o[x] * by;
-  if (p.weights && lane == 0) {
-    float* stats = static_cast<float*>(p.scratch) + plan.stats + (head * rows + row) * 2;
-    stats[0] = base;
-    stats[1] = by;
-  }
+  for (int c = 0; c < 4; ++c)
+    if (c * 64 + lane < p.dhead) to[c * 64 + lane] = total == 0.f ? 0.f : o[c] * by;
 }
 
 // weights[b, hkv, t] += sum over the group's heads of exp(s_t - m) / l
-__global__ __launch_bounds__(kThreads) void cache_weights_kernel(CacheAttnParams p, CachePlan plan) {
-  const int64_t tiles = (p.t_max + kThreads - 1) / kThreads, unit = blockIdx.x / tiles;
-  const int64_t group = p.heads / p.heads_kv;
-  const int len = committed(p, unit / p.heads_kv);
-  const int64_t t = blockIdx.x % tiles * kThreads + threadIdx.x;
-  if (t >= len) return;
-  const float* scores = static_cast<const float*>(p.scratch) + plan.scores + unit * group * plan.score_pitch;
-  const float* stats = static_cast<const float*>(p.scratch) + plan.stats + unit * group * 2;
-  float sum = 0.f;
-  for (int64_t r = 0; r < group; ++r)
-    sum += __builtin_amdgcn_exp2f(scores[r * plan.score_pitch + t] - stats[2 * r]) * stats[2 * r + 1];
-  p.weights[unit * p.t_max + t] += sum;
+constexpr int kWeightSteps = 4;  // positions of a thread
+__device__ void add_weights(const CacheAttnParams& p, const CachePlan& plan, int64_t index) {
+  __shared__ v2f stats_s[1024];
+  const int64_t head = index / plan.weight_tiles;
+  const int t0 = static_cast<int>(index - head * plan.weight_tiles) * kThreads * kWeightSteps + threadIdx.x;
+  const int group = static_cast<int>(p.heads / p.heads_kv);
+  const int len = committed(p, head / p.heads_kv);
+  if (t0 - static_cast<int>(threadIdx.x) >= len) return;
+  const float* scratch = static_cast<const float*>(p.scratch);
+  for (int r = threadIdx.x; r < group; r += kThreads) {
+    v2f stats = reinterpret_cast<const v2f*>(scratch + plan.stats)[head * group + r];
+    if (!plan.whole) {
+      const Parts parts(p, plan, head * plan.row_groups + r / plan.unit_rows);
+      if (parts.count > 1) {
+        const int local = r % plan.unit_rows;
+        const v2f* ml = reinterpret_cast<const v2f*>(scratch + plan.parts_ml);
+        float most = -INFINITY, total = 0.f;
+        for (int i = 0; i < parts.count; ++i) most = fmaxf(most, ml[parts.row(plan, i, local)][0]);
+        const float base = finite_base(most);
+        for (int i = 0; i < parts.count; ++i) {
+          const v2f part = ml[parts.row(plan, i, local)];
+          total += part[1] * shift_of(part[0], base);
+        }
+        stats = v2f{base, total == 0.f ? 0.f : 1.f / total};
+      }
+    }
+    stats_s[r] = stats;
+  }
+  __syncthreads();
+  const float* scores = scratch + plan.scores + head * group * plan.score_pitch;
+  float* weights = p.weights + head * p.t_max;
+  float sum[kWeightSteps], old[kWeightSteps];
+#pragma unroll
+  for (int u = 0; u < kWeightSteps; ++u) {
+    sum[u] = 0.f;
+    old[u] = t0 + u * kThreads < len ? weights[t0 + u * kThreads] : 0.f;
+  }
+#pragma unroll 2
+  for (int r = 0; r < group; ++r) {
+    const v2f stats = stats_s[r];
+#pragma unroll
+    for (int u = 0; u < kWeightSteps; ++u) {
+      const int t = t0 + u * kThreads < len ? t0 + u * kThreads : 0;
+      sum[u] += __builtin_amdgcn_exp2f(scores[r * plan.score_pitch + t] - stats[0]) * stats[1];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kWeightSteps; ++u)
+    if (t0 + u * kThreads < len) weights[t0 + u * kThreads] = old[u] + sum[u];
+}
+
+__global__ __launch_bounds__(kThreads) void finish_kernel(CacheAttnParams p, CachePlan plan) {
+  if (blockIdx.x < static_cast<unsigned>(plan.join_groups)) join_rows(p, plan);
+  else add_weights(p, plan, blockIdx.x - plan.join_groups);
 }
 
 // ---- the host's side -------------------------------------------------------------------------
@@ -796,12 +861,13 @@ CachePlan make_plan(const CacheAttnParams& p) {
   plan.min_rounds = plan.row_waves == 1 ? 4 : 8;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  plan.whole = walked <= plan.round_keys * plan.min_rounds || units >= 2048;
+  plan.whole = walked <= plan.round_keys * 16 || units >= 2048;
   // scratch
   auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;
-  plan.parts_ml = 0;
-  plan.parts_o = up(parts * 2);
+  plan.records = 0;
+  plan.parts_ml = plan.whole ? 0 : up(units * 2);
+  plan.parts_o = plan.parts_ml + up(parts * 2);
   plan.stats = plan.parts_o + up(parts * p.dhead);
   plan.scores = plan.stats;
   plan.total = plan.stats;
@@ -811,6 +877,9 @@ CachePlan make_plan(const CacheAttnParams& p) {
     plan.scores = plan.stats + up(p.batch * p.heads * 2);
     plan.total = plan.scores + p.batch * p.heads * plan.score_pitch;
   }
+  plan.join_groups = plan.whole ? 0 : static_cast<int>((units * plan.unit_rows + kWaves - 1) / kWaves);
+  plan.weight_tiles =
+      p.weights ? static_cast<int>((p.t_max + kThreads * kWeightSteps - 1) / (kThreads * kWeightSteps)) : 0;
   return plan;
 }
 
@@ -858,13 +927,9 @@ void launch_cache_attention(const CacheAttnParams& p, hipStream_t stream) {
   if (p.kv_dtype == kF32) launch_typed<kF32>(p, plan, stream);
   else if (p.kv_dtype == kF16) launch_typed<kF16>(p, plan, stream);
   else launch_typed<kBF16>(p, plan, stream);
-  if (!plan.whole)
-    hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>(p.batch * p.tokens * p.heads)), dim3(64), 0, stream, p,
-                       plan);
-  if (p.weights)
-    hipLaunchKernelGGL(cache_weights_kernel,
-                       dim3(static_cast<unsigned>((p.t_max + kThreads - 1) / kThreads * p.batch * p.heads_kv)),
-                       dim3(kThreads), 0, stream, p, plan);
+  const int64_t finish = plan.join_groups + plan.weight_tiles * p.batch * p.heads_kv;
+  if (finish)
+    hipLaunchKernelGGL(finish_kernel, dim3(static_cast<unsigned>(finish)), dim3(kThreads), 0, stream, p, plan);
 }
 
 }  // namespace ct2x
