@@ -57,6 +57,8 @@ constexpr int kF32 = 0, kF16 = 4, kBF16 = 5;
 
 // How a launch cuts its work; the same on the host and in every kernel of a call.
 struct CachePlan {
+  bool shared;      // positions shared through LDS
+  int tiles;        // tiles of 16 rows of a wave
   int row_waves;    // waves of a workgroup that take different rows; the others share rows and take
                     // different positions
   int unit_rows;    // rows of a unit
@@ -164,12 +166,9 @@ struct Mfma {  // 16-bit
   }
 };
 
-template <int kType>
-__device__ __forceinline__ float element(const void* base, int64_t i) {
-  if constexpr (kType == kF32) return static_cast<const float*>(base)[i];
-  else if constexpr (kType == kF16) return __half2float(static_cast<const __half*>(base)[i]);
-  else return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[i]) << 16);
-}
+// Keeps what is computed from x where it is written: not moved out of a loop or a branch that is
+// seldom taken, where it would hold registers all along.
+__device__ __forceinline__ void rare(int& x) { asm volatile("" : "+v"(x)); }
 
 // the larger / the sum over the four lanes of a row (lanes c, c + 16, c + 32, c + 48)
 __device__ __forceinline__ float rows_max(float x) {
@@ -201,19 +200,28 @@ struct Tile {
   static constexpr int H = DP / (16 * W);                    // V: loads per position and lane
   static constexpr int E = H * W;                            // output tiles of 16 channels
   static constexpr int kWords = W * kBytes / 4;              // registers of a V load
+  // shared tiles of keys / of values in LDS
+  static constexpr int kTileBytes = 16384;
+  static constexpr int kTileKeys = kTileBytes / (DP * kBytes);
+  static constexpr int kRowChunks = DP * kBytes / 16;
 };
+
+typedef __attribute__((address_space(3))) void lds_void;
 
 // ---- the kernel ------------------------------------------------------------------------------
 
-template <int kType, int DP, int NT, CacheView kView>
+// kShared: the four waves take different rows of the same positions; keys and values come from tiles in
+// LDS that the workgroup fills, one ahead of the one in use.
+template <int kType, int DP, int NT, CacheView kView, bool kShared>
 struct Worker {
   using T = Tile<kType, DP, NT>;
   const CacheAttnParams& p;
   const CachePlan& plan;
-  float* lds;  // 2 x NT x (E x 4 + 2) x 64 floats
+  char* lds;  // join_waves: 2 x NT x (E x 4 + 2) x 64 floats; kShared: 2 x (keys, values) tiles
   int lane, g, c, wave_r, wave_k, key_waves;
   int group, rows, row_bytes;
-  uint32_t k_channel[T::kChunks], v_channel[T::H];  // byte offsets of the lane's channels in a row
+  // byte offsets of the lane's channels in a row (kShared: of LDS)
+  uint32_t k_channel[T::kChunks], v_channel[T::H];
 
   // the unit
   int64_t b;
@@ -231,7 +239,7 @@ struct Worker {
   v4u k[T::kKeyTiles][T::kChunks];
   uint32_t v[T::kLane][T::H][T::kWords];
 
-  __device__ __forceinline__ Worker(const CacheAttnParams& p, const CachePlan& plan, float* lds)
+  __device__ __forceinline__ Worker(const CacheAttnParams& p, const CachePlan& plan, char* lds)
       : p(p), plan(plan), lds(lds) {
     lane = threadIdx.x & 63;
     g = lane >> 4;
@@ -248,12 +256,13 @@ struct Worker {
 #pragma unroll
     for (int s = 0; s < T::kChunks; ++s) {
       const int byte = s * 64 + g * 16;
-      k_channel[s] = byte < row_bytes ? byte : kNoChannel;
+      if constexpr (kShared) k_channel[s] = ((s * 4 + g) ^ c) % T::kRowChunks * 16;
+      else k_channel[s] = byte < row_bytes ? byte : kNoChannel;
     }
 #pragma unroll
     for (int h = 0; h < T::H; ++h) {
       const int byte = (h * 16 + c) * T::W * T::kBytes;
-      v_channel[h] = byte < row_bytes ? byte : kNoChannel;
+      v_channel[h] = kShared || byte < row_bytes ? byte : kNoChannel;
     }
   }
 
@@ -383,15 +392,79 @@ struct Worker {
       }
   }
 
-  // does row `row` see walked position t (at: its cache position)?
-  __device__ __forceinline__ bool sees(int row, int at) const {
-    if (at < 0) return false;
-    if (at < len) return true;
-    if (kView != CacheView::kTree || at >= end || row >= rows) return false;
-    const int j = at - len, i = row / group;
-    if (!p.mask) return j <= i;
-    const int words = (static_cast<int>(p.tokens) + 63) / 64;
-    return (p.mask[(b * p.tokens + i) * words + (j >> 6)] >> (j & 63)) & 1;
+  // Tiles of positions t .. t + kTileKeys - 1 on their way into LDS, 16 bytes per lane and request.
+  // Loads fill LDS in lane order, so the keys' swizzle - a row's 16-byte units are permuted by the
+  // number of the lane that will read it as its A row, which puts the 16 rows that lanes read
+  // together on all banks - is made by what a lane asks for.
+  __device__ __forceinline__ void stage(int t, int buffer) {
+    constexpr int kLoads = T::kTileBytes / (kThreads * 16);
+    int thread = threadIdx.x;
+    rare(thread);  // (the offsets are made again per tile: kept, they would cost the registers of a row tile)
+    char* to = lds + buffer * 2 * T::kTileBytes + uniform(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * kThreads + thread, row = at / T::kRowChunks, unit = at % T::kRowChunks;
+      const int reader = T::kHalf ? (row & 3) | (row >> 3 & 3) << 2 : row & 15;
+      const int k_byte = (unit ^ (reader % T::kRowChunks)) * 16, v_byte = unit * 16;
+      const uint32_t from = static_cast<uint32_t>(t + row) * static_cast<uint32_t>(row_bytes);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(k_rsrc, (lds_void*)(to + i * kThreads * 16), 16,
+                                               from + (k_byte < row_bytes ? k_byte : kNoChannel), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(v_rsrc, (lds_void*)(to + T::kTileBytes + i * kThreads * 16), 16,
+                                               from + (v_byte < row_bytes ? v_byte : kNoChannel), 0, 0, 0);
+    }
+  }
+
+  // the step's keys / values from the tile; `first`: its first row there
+  __device__ __forceinline__ void read_keys(const char* tile, int first) {
+#pragma unroll
+    for (int i = 0; i < T::kKeyTiles; ++i) {
+      const int row = first + (T::kHalf ? (c >> 2) * 8 + i * 4 + (c & 3) : c);
+#pragma unroll
+      for (int s = 0; s < T::kChunks; ++s)
+        k[i][s] = *reinterpret_cast<const v4u*>(tile + row * DP * T::kBytes + k_channel[s]);
+    }
+  }
+  __device__ __forceinline__ void read_values(const char* tile, int first) {
+#pragma unroll
+    for (int j = 0; j < T::kLane; ++j)
+#pragma unroll
+      for (int h = 0; h < T::H; ++h) {
+        const char* from = tile + (first + g * T::kLane + j) * DP * T::kBytes + v_channel[h];
+        if constexpr (T::kWords == 4) {
+          const v4u x = *reinterpret_cast<const v4u*>(from);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[j][h][w] = x[w];
+        } else {
+          const v2u x = *reinterpret_cast<const v2u*>(from);
+          v[j][h][0] = x[0];
+          v[j][h][1] = x[1];
+        }
+      }
+  }
+
+  // bit j: row `row` does not see cache position at + j (at < 0: there is none)
+  __device__ __forceinline__ uint32_t hidden_from(int row, int at) const {
+    constexpr uint32_t kAll = (1u << T::kLane) - 1;
+    if (at < 0) return kAll;
+    const uint32_t old = at + T::kLane <= len ? kAll : at < len ? (1u << (len - at)) - 1 : 0u;
+    if (kView != CacheView::kTree || row >= rows) return kAll & ~old;
+    const int first = at - len, i = row / group, tokens = static_cast<int>(p.tokens);  // drafted token of bit 0
+    uint32_t seen = 0u;
+    if (!p.mask) {  // tokens up to i
+      const int upto = i + 1 - first;
+      seen = upto >= T::kLane ? kAll : upto > 0 ? (1u << upto) - 1 : 0u;
+    } else {
+      const int words = (tokens + 63) / 64;
+      const uint64_t* mask = p.mask + (b * tokens + i) * words;
+#pragma unroll
+      for (int j = 0; j < T::kLane; ++j) {
+        const int token = first + j;
+        if (token >= 0 && token < tokens) seen |= static_cast<uint32_t>(mask[token >> 6] >> (token & 63) & 1) << j;
+      }
+    }
+    const int there = end - at;  // (positions behind the last drafted token)
+    if (there < T::kLane) seen &= there > 0 ? (1u << there) - 1 : 0u;
+    return kAll & ~(old | seen);
   }
 
   __device__ __forceinline__ bool values_finite() const {
@@ -414,8 +487,11 @@ struct Worker {
   }
 
   // one step over positions step .. step + kStep - 1, whose keys and values are in registers or on
-  // their way; `next` is loaded as their registers come free
-  __device__ __forceinline__ void advance(int step, int next) {
+  // their way; `next` is loaded as their registers come free (kShared: they are in `tile`). kPlain: all
+  // positions are committed ones, every row sees them.
+  template <bool kPlain>
+  __device__ __forceinline__ void advance(int step, int next, const char* tile = nullptr, int first = 0) {
+    if constexpr (kShared) read_keys(tile, first);
     float s[NT][T::kLane];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -440,22 +516,27 @@ struct Worker {
         for (int j = 0; j < 4; ++j) s[n][i * 4 + j] = acc[j] * factor[n];
       }
     }
-    load_keys(next);
+    if constexpr (kShared) read_values(tile + T::kTileBytes, first);
+    else load_keys(next);
 
-    const int at = position(step + g * T::kLane);
-    const bool full = __all(at >= 0 && at + T::kLane <= len);
     uint32_t hidden[NT];  // bit j: the row does not see the lane's position j
+    bool full = true;
+    if constexpr (!kPlain) {
+      const int at = position(step + g * T::kLane);
+      full = __all(at >= 0 && at + T::kLane <= len);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) hidden[n] = 0u;
-    if (!full) {
+      for (int n = 0; n < NT; ++n) hidden[n] = 0u;
+      if (!full) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          int row = row0 + n * 16 + c;
+          rare(row);
+          hidden[n] = hidden_from(row, at);
 #pragma unroll
-        for (int j = 0; j < T::kLane; ++j)
-          if (!sees(row0 + n * 16 + c, at < 0 ? -1 : at + j)) {
-            s[n][j] = -INFINITY;
-            hidden[n] |= 1u << j;
-          }
+          for (int j = 0; j < T::kLane; ++j)
+            if (hidden[n] >> j & 1) s[n][j] = -INFINITY;
+        }
+      }
     }
     if (kView == CacheView::kDense && p.weights) {
       // the scores (times log2 e) wait for the row's statistics; the rows' pitch is a multiple of a step
@@ -493,9 +574,17 @@ struct Worker {
       }
     }
 
-    if (kView == CacheView::kTree && !full && !__all(values_finite())) {
-      add_values_apart(step, s, hidden);
-    } else if constexpr (T::kHalf) {
+    bool apart = false;
+    if constexpr (kView == CacheView::kTree && !kPlain) {
+      apart = !full && !__all(values_finite());
+      if (apart) add_values_apart(step, s, hidden);
+    }
+    if (!apart) add_values(s);
+    if constexpr (!kShared) load_values(next);
+  }
+
+  __device__ __forceinline__ void add_values(const float (&s)[NT][T::kLane]) {
+    if constexpr (T::kHalf) {
       v4u hi[NT], lo[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -532,7 +621,6 @@ struct Worker {
               o[n][h * T::W + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][h][e]), s[n][j],
                                                                         o[n][h * T::W + e], 0, 0, 0);
     }
-    load_values(next);
   }
 
   // A drafted position holds NaN or infinite values that some rows must not see: 0 x inf would reach
@@ -542,41 +630,94 @@ struct Worker {
     for (int key = 0; key < T::kStep; ++key) {
       const int at = step + key, from = key / T::kLane * 16 + c, j = key % T::kLane;
       if (at >= end) break;
+      const uint32_t row = byte_of(at);
+      float x[NT];
+      bool seen[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float x = s[n][0];
+        x[n] = s[n][0];
 #pragma unroll
-        for (int i = 1; i < T::kLane; ++i) x = j == i ? s[n][i] : x;
-        x = __shfl(x, from);
-        const bool seen = !(__shfl(hidden[n], from) >> j & 1);
-#pragma unroll
-        for (int h = 0; h < T::H; ++h)
-#pragma unroll
-          for (int e = 0; e < T::W; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int d = (h * 16 + g * 4 + i) * T::W + e;
-              if (seen && d < p.dhead)
-                o[n][h * T::W + e][i] = fmaf(x, element<kType>(v_base, static_cast<int64_t>(at) * p.dhead + d),
-                                             o[n][h * T::W + e][i]);
-            }
+        for (int i = 1; i < T::kLane; ++i) x[n] = j == i ? s[n][i] : x[n];
+        x[n] = __shfl(x[n], from);
+        seen[n] = !(__shfl(hidden[n], from) >> j & 1);
       }
+#pragma unroll
+      for (int h = 0; h < T::H; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // channels behind dhead read as zeros or as other channels: they are not stored
+          const uint32_t byte = row + (h * 16 + g * 4 + i) * T::W * T::kBytes;
+          v2u y[T::kWords / 2];
+#pragma unroll
+          for (int w = 0; w < T::kWords / 2; ++w)
+            y[w] = __builtin_amdgcn_raw_buffer_load_b64(v_rsrc, byte + 8 * w, 0, 0);
+#pragma unroll
+          for (int e = 0; e < T::W; ++e) {
+            float value;
+            if constexpr (kType == kF32) {
+              value = __uint_as_float(y[e >> 1][e & 1]);
+            } else {
+              const uint32_t bits = e & 1 ? y[e >> 2][e >> 1 & 1] >> 16 : y[e >> 2][e >> 1 & 1] & 0xffffu;
+              if constexpr (kType == kF16) value = __builtin_bit_cast(v2h, bits)[0];
+              else value = __uint_as_float(bits << 16);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float sum = fmaf(x[n], value, o[n][h * T::W + e][i]);
+              o[n][h * T::W + e][i] = seen[n] ? sum : o[n][h * T::W + e][i];
+            }
+          }
+        }
     }
   }
 
-  // rounds r0 .. r1 - 1 of the unit
+  // the tile of round r, once it has arrived; the next one is requested before it is used
+  template <bool kPlain>
+  __device__ __forceinline__ void advance_tile(int r, int r0, int r1) {
+    // this tile has arrived and the other one is read: no later request may still be under way here
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (r + 1 < r1) stage((r + 1) * T::kTileKeys, (r + 1 - r0) & 1);
+    const char* tile = lds + ((r - r0) & 1) * 2 * T::kTileBytes;
+#pragma unroll 1
+    for (int i = 0; i < T::kTileKeys; i += T::kStep)
+      if (kPlain || r * T::kTileKeys + i < end) advance<kPlain>(r * T::kTileKeys + i, 0, tile, i);
+  }
+
+  // rounds r0 .. r1 - 1 of the unit: those over committed positions alone first (the loop that counts
+  // keeps the masks' code and registers out)
   __device__ __forceinline__ void walk(int r0, int r1) {
-    auto first = [&](int r) {
-      const int t = r * plan.round_keys + wave_k * T::kStep;
-      return r < r1 && t < end ? t : -1;
-    };
-    int step = first(r0);
-    load_keys(step);
-    load_values(step);
-    for (int r = r0; step >= 0; ++r) {
-      const int next = first(r + 1);
-      advance(step, next);
-      step = next;
+    if constexpr (kShared) {
+      __syncthreads();  // nobody reads the tiles of the unit before
+      stage(r0 * T::kTileKeys, 0);
+      const int plain = len / T::kTileKeys;
+      int r = r0;
+#pragma unroll 1
+      for (; r < r1 && r < plain; ++r) advance_tile<true>(r, r0, r1);
+#pragma unroll 1
+      for (; r < r1; ++r) advance_tile<false>(r, r0, r1);
+    } else {
+      auto first = [&](int r) {
+        const int t = r * plan.round_keys + wave_k * T::kStep;
+        return r < r1 && t < end ? t : -1;
+      };
+      int step = first(r0), r = r0;
+      load_keys(step);
+      load_values(step);
+      if constexpr (kView != CacheView::kBlocks) {
+#pragma unroll 1
+        for (; step >= 0 && step + T::kStep <= len; ++r) {
+          const int next = first(r + 1);
+          advance<true>(step, next);
+          step = next;
+        }
+      }
+#pragma unroll 1
+      for (; step >= 0; ++r) {
+        const int next = first(r + 1);
+        advance<false>(step, next);
+        step = next;
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) l[n] = rows_sum(l[n]);
@@ -586,7 +727,7 @@ struct Worker {
   __device__ __forceinline__ void join_waves() {
     constexpr int kFloats = NT * (T::E * 4 + 2) * 64;
     for (int half = key_waves / 2; half >= 1; half /= 2) {
-      float* mine = lds + (wave_r * half + wave_k % half) * kFloats;
+      float* mine = reinterpret_cast<float*>(lds) + (wave_r * half + wave_k % half) * kFloats;
       __syncthreads();
       if (wave_k >= half && wave_k < 2 * half) {
 #pragma unroll
@@ -621,7 +762,7 @@ struct Worker {
 
   // the unit's outputs, or a part's (m, l, o)
   __device__ __forceinline__ void finish(bool complete, int64_t part) {
-    if (key_waves > 1) join_waves();
+    if (!kShared && key_waves > 1) join_waves();
     if (wave_k != 0) return;
     float* scratch = static_cast<float*>(p.scratch);
 #pragma unroll
@@ -657,46 +798,51 @@ struct Worker {
   }
 };
 
-constexpr int waves_per_simd(int type, int dp, int nt) { return dp * nt >= 256 ? 1 : 2; }
+constexpr int waves_per_simd(int dp, int nt, bool shared) {
+  return dp == 256 || (dp * nt == 256 && !shared) ? 1 : 2;
+}
 
-template <int kType, int DP, int NT, CacheView kView>
-__global__ __launch_bounds__(kThreads, waves_per_simd(kType, DP, NT))
+template <int kType, int DP, int NT, CacheView kView, bool kShared>
+__global__ __launch_bounds__(kThreads, waves_per_simd(DP, NT, kShared))
 void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
-  extern __shared__ float lds[];
-  Worker<kType, DP, NT, kView> worker(p, plan, lds);
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  Worker<kType, DP, NT, kView, kShared> worker(p, plan, lds);
   const int units = static_cast<int>(p.heads_kv) * plan.row_groups;
-  if (plan.whole) {
-    const int64_t b = blockIdx.x / units;
-    worker.begin(b, blockIdx.x % units);
-    worker.walk(0, uniform(rounds_of(p, plan, b)));
-    worker.finish(true, 0);
-    return;
-  }
-  const Line line = make_line(p, plan);
-  if (blockIdx.x >= line.groups) return;
-  int64_t x = line.start(blockIdx.x);
-  const int64_t x0 = x, x1 = line.start(blockIdx.x + 1);
-  // the entry that x lies in: 64 entries at a time
-  int64_t b = 0, before = 0;
-  for (;; b += 64) {
-    const int lane = threadIdx.x & 63;
-    const int64_t mine = b + lane < p.batch ? static_cast<int64_t>(rounds_of(p, plan, b + lane)) * units : 0;
-    int64_t upto = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t y = __shfl_up(static_cast<long long>(upto), o, 64);
-      if (lane >= o) upto += y;
+  Line line{0, 0, 1, 0};
+  int64_t b = 0, before = 0, x, x1;  // entry, the round of the line that it begins at, the stretch
+  if (plan.whole) {  // a line of the one entry
+    b = blockIdx.x / units;
+    const int n = uniform(rounds_of(p, plan, b));
+    x = static_cast<int64_t>(blockIdx.x % units) * n;
+    x1 = x + n;
+  } else {
+    line = make_line(p, plan);
+    if (blockIdx.x >= line.groups) return;
+    x = line.start(blockIdx.x);
+    x1 = line.start(blockIdx.x + 1);
+    // the entry that x lies in: 64 entries at a time
+    for (;; b += 64) {
+      const int lane = threadIdx.x & 63;
+      const int64_t mine = b + lane < p.batch ? static_cast<int64_t>(rounds_of(p, plan, b + lane)) * units : 0;
+      int64_t upto = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(static_cast<long long>(upto), o, 64);
+        if (lane >= o) upto += y;
+      }
+      const uint64_t behind = __ballot(before + upto > x);
+      if (behind) {
+        const int at = __builtin_ctzll(behind);
+        before += __shfl(static_cast<long long>(upto - mine), at);
+        b += at;
+        break;
+      }
+      before += __shfl(static_cast<long long>(upto), 63);
     }
-    const uint64_t behind = __ballot(before + upto > x);
-    if (behind) {
-      const int at = __builtin_ctzll(behind);
-      before += __shfl(static_cast<long long>(upto - mine), at);
-      b += at;
-      break;
-    }
-    before += __shfl(static_cast<long long>(upto), 63);
+    b = uniform64(b);
+    before = uniform64(before);
   }
-  b = uniform64(b);
-  before = uniform64(before);
+  const int64_t x0 = x;
+#pragma unroll 1
   while (x < x1) {
     const int n = uniform(rounds_of(p, plan, b));
     const int64_t within = x - before;
@@ -706,7 +852,7 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
     worker.walk(r0, r1);
     // a part that begins the workgroup's stretch is its first, any other its last
     const int slot = blockIdx.x * 2 + (x == x0 ? 0 : 1);
-    if (r0 == 0 && threadIdx.x == 0) {
+    if (!plan.whole && r0 == 0 && threadIdx.x == 0) {
       const int count = static_cast<int>(line.holder(x + n - 1)) - static_cast<int>(blockIdx.x) + 1;
       reinterpret_cast<int2*>(static_cast<float*>(p.scratch) + plan.records)[b * units + unit] = int2{slot, count};
     }
@@ -845,23 +991,23 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(CacheAttnParams p, Cac
 
 int padded_head(int64_t dhead) { return dhead <= 64 ? 64 : (dhead <= 128 ? 128 : 256); }
 
-int row_tiles(const CacheAttnParams& p, int64_t rows) {
-  return rows <= 16 || p.view != CacheView::kTree || padded_head(p.dhead) == 256 ? 1 : 2;
-}
-
 CachePlan make_plan(const CacheAttnParams& p) {
   CachePlan plan;
   const int64_t rows = p.tokens * (p.heads / p.heads_kv);
-  const int tiles = row_tiles(p, rows);
-  plan.row_waves = rows <= 16 * tiles ? 1 : (rows <= 32 * tiles ? 2 : 4);
-  plan.unit_rows = 16 * tiles * plan.row_waves;
+  const int dp = padded_head(p.dhead), element = p.kv_dtype == kF32 ? 4 : 2;
+  // Few rows: every wave takes all of them and its own positions. From 33 on: a wave has its own 16 or
+  // 32, and the positions are shared through LDS.
+  plan.shared = p.view == CacheView::kTree && rows > 32;
+  plan.tiles = p.view != CacheView::kTree || rows <= 16 || dp == 256 || (plan.shared && rows <= 64) ? 1 : 2;
+  plan.row_waves = plan.shared || rows > 32 * plan.tiles ? 4 : (rows > 16 * plan.tiles ? 2 : 1);
+  plan.unit_rows = 16 * plan.tiles * plan.row_waves;
   plan.row_groups = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
-  plan.round_keys = (p.kv_dtype == kF32 ? 16 : 32) * (kWaves / plan.row_waves);
+  plan.round_keys = plan.shared ? 16384 / (dp * element) : (element == 4 ? 16 : 32) * (kWaves / plan.row_waves);
   plan.grid = 512;
-  plan.min_rounds = plan.row_waves == 1 ? 4 : 8;
+  plan.min_rounds = 4;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  plan.whole = walked <= plan.round_keys * 16 || units >= 2048;
+  plan.whole = walked <= plan.round_keys * 8 || units >= 2048;
   // scratch
   auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;
@@ -883,13 +1029,13 @@ CachePlan make_plan(const CacheAttnParams& p) {
   return plan;
 }
 
-template <int kType, int DP, int NT, CacheView kView>
+template <int kType, int DP, int NT, CacheView kView, bool kShared = false>
 void launch_tiles(const CacheAttnParams& p, const CachePlan& plan, hipStream_t stream) {
   using T = Tile<kType, DP, NT>;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  const int key_waves = kWaves / plan.row_waves;
-  const size_t lds = key_waves > 1 ? sizeof(float) * (kWaves / 2) * NT * (T::E * 4 + 2) * 64 : 0;
-  hipLaunchKernelGGL((cache_attention_kernel<kType, DP, NT, kView>),
+  const size_t lds = kShared ? 4 * T::kTileBytes
+                             : plan.row_waves < kWaves ? sizeof(float) * (kWaves / 2) * NT * (T::E * 4 + 2) * 64 : 0;
+  hipLaunchKernelGGL((cache_attention_kernel<kType, DP, NT, kView, kShared>),
                      dim3(static_cast<unsigned>(plan.whole ? units : plan.grid)), dim3(kThreads), lds, stream, p, plan);
 }
 
@@ -898,9 +1044,12 @@ void launch_head(const CacheAttnParams& p, const CachePlan& plan, hipStream_t st
   if (p.view == CacheView::kDense) return launch_tiles<kType, DP, 1, CacheView::kDense>(p, plan, stream);
   if (p.view == CacheView::kBlocks) return launch_tiles<kType, DP, 1, CacheView::kBlocks>(p, plan, stream);
   if constexpr (DP < 256) {
-    if (plan.unit_rows / plan.row_waves == 32) return launch_tiles<kType, DP, 2, CacheView::kTree>(p, plan, stream);
+    if (plan.tiles == 2)
+      return plan.shared ? launch_tiles<kType, DP, 2, CacheView::kTree, true>(p, plan, stream)
+                         : launch_tiles<kType, DP, 2, CacheView::kTree>(p, plan, stream);
   }
-  launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
+  if (plan.shared) launch_tiles<kType, DP, 1, CacheView::kTree, true>(p, plan, stream);
+  else launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
 }
 
 template <int kType>
