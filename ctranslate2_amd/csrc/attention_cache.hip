@@ -310,16 +310,16 @@ struct Worker {
           const int d = s * 32 + g * 8;
           const bool there = row < rows && d < p.dhead;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            v4f y = {0.f, 0.f, 0.f, 0.f};
-            if (there) y = *reinterpret_cast<const v4f*>(q + d + 4 * i);
+          for (int i = 0; i < 2; ++i) {  // (loads without a branch: all are requested before the first is used)
+            const v4f y = *reinterpret_cast<const v4f*>(q + (d < p.dhead ? d : 0) + 4 * i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[s][4 * i + j] = y[j];
-              most = fmaxf(most, fabsf(y[j]));
-            }
+            for (int j = 0; j < 4; ++j) x[s][4 * i + j] = there ? y[j] : 0.f;
           }
         }
+#pragma unroll
+        for (int s = 0; s < T::kChunks; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[s][j]));
         // to [1, 2) by a power of two, which the factor takes back: float16 has no room for less or more
         const int power = ilogbf(fmaxf(rows_max(most), 1.17549435e-38f));
         const int shift = power > 126 ? 126 : power;
@@ -335,10 +335,10 @@ struct Worker {
 #pragma unroll
         for (int s = 0; s < T::kChunks; ++s) {
           const int d = s * 16 + g * 4;
-          v4f y = {0.f, 0.f, 0.f, 0.f};
-          if (row < rows && d < p.dhead) y = *reinterpret_cast<const v4f*>(q + d);
+          const v4f y = *reinterpret_cast<const v4f*>(q + (d < p.dhead ? d : 0));
+          const bool there = row < rows && d < p.dhead;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = __float_as_uint(y[j]);
+          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = there ? __float_as_uint(y[j]) : 0u;
         }
       }
     }
@@ -454,13 +454,12 @@ struct Worker {
       const int upto = i + 1 - first;
       seen = upto >= T::kLane ? kAll : upto > 0 ? (1u << upto) - 1 : 0u;
     } else {
-      const int words = (tokens + 63) / 64;
+      const int words = (tokens + 63) / 64, from = first < 0 ? 0 : first, word = from >> 6;
       const uint64_t* mask = p.mask + (b * tokens + i) * words;
-#pragma unroll
-      for (int j = 0; j < T::kLane; ++j) {
-        const int token = first + j;
-        if (token >= 0 && token < tokens) seen |= static_cast<uint32_t>(mask[token >> 6] >> (token & 63) & 1) << j;
-      }
+      const uint64_t low = mask[word < words ? word : 0], high = mask[word + 1 < words ? word + 1 : 0];
+      const int shift = from & 63;
+      const uint64_t bits = low >> shift | (shift ? high << (64 - shift) : 0ull);
+      seen = first > -T::kLane ? static_cast<uint32_t>(bits << (from - first)) & kAll : 0u;
     }
     const int there = end - at;  // (positions behind the last drafted token)
     if (there < T::kLane) seen &= there > 0 ? (1u << there) - 1 : 0u;
