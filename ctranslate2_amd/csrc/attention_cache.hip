@@ -29,6 +29,8 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "cache_ops.h"
 #include "device_utils.h"
@@ -46,8 +48,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
+constexpr int kThreads = 256;  // of a workgroup whose waves load for themselves; shared tiles: 512
+constexpr int waves_of(bool shared) { return shared ? 8 : 4; }
 constexpr float kLog2e = 1.44269504088896340736f;
 // Buffer offsets that are out of range of every head's region (at most 2^31 - 2^20 bytes), the load
 // returns zeros: of a row that is not there, and of channels behind dhead; their sum does not wrap.
@@ -82,7 +84,10 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 
 __device__ __forceinline__ int committed(const CacheAttnParams& p, int64_t b) {
   const int64_t room = p.t_max - (p.view == CacheView::kTree ? p.tokens : 0);
-  const int64_t n = p.lengths ? p.lengths[b] : p.length;
+  // (by the scalar cache where b is the wave's)
+  const auto* lengths = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+      reinterpret_cast<uintptr_t>(p.lengths));
+  const int64_t n = p.lengths ? lengths[b] : p.length;
   return static_cast<int>(n < 0 ? 0 : (n > room ? room : n));
 }
 
@@ -101,43 +106,32 @@ __device__ __forceinline__ int rounds_of(const CacheAttnParams& p, const CachePl
   return n < 1 ? 1 : n;
 }
 
-// a / b of what fits 32 bits in all but the largest calls
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  if ((a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
-}
-
 // The line of all rounds and how many workgroups share it: the first `longer` take `each` + 1 rounds.
+// (A line has less than 2048 units - launch_cache_attention - of at most 2^20 rounds.)
 struct Line {
-  int64_t total, groups, each, longer;
-  __device__ __forceinline__ int64_t start(int64_t w) const { return w * each + (w < longer ? w : longer); }
+  uint32_t total, groups, each, longer;
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * each + (w < longer ? w : longer); }
   // the workgroup that holds round x
-  __device__ __forceinline__ int64_t holder(int64_t x) const {
-    const int64_t ahead = longer * (each + 1);
-    return x < ahead ? divide(x, each + 1) : longer + divide(x - ahead, each);
+  __device__ __forceinline__ uint32_t holder(uint32_t x) const {
+    const uint32_t ahead = longer * (each + 1);
+    return x < ahead ? x / (each + 1) : longer + (x - ahead) / each;
   }
 };
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(static_cast<long long>(x), o, 64);
+// sums over the lanes up to each
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  auto moved = [&](auto ctrl, auto rows) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x += moved(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // 1, 2, 4, 8 to the right in a row
+  x += moved(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // the rows before, summed
+  x += moved(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
   return x;
-}
-
-// rounds of the units of entries 0 .. entries - 1 (per unit of an entry: times units)
-__device__ __forceinline__ int64_t rounds_before(const CacheAttnParams& p, const CachePlan& plan, int64_t entries) {
-  int64_t sum = 0;
-  for (int64_t b = threadIdx.x & 63; b < entries; b += 64) sum += rounds_of(p, plan, b);
-  return uniform64(wave_sum64(sum)) * p.heads_kv * plan.row_groups;
-}
-
-__device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CachePlan& plan) {
-  Line line;
-  line.total = rounds_before(p, plan, p.batch);
-  const int64_t groups = divide(line.total, plan.min_rounds);
-  line.groups = groups < 1 ? 1 : (groups > plan.grid ? plan.grid : groups);
-  line.each = divide(line.total, line.groups);
-  line.longer = line.total - line.each * line.groups;
-  return line;
 }
 
 // ---- the types -------------------------------------------------------------------------------
@@ -218,7 +212,8 @@ struct Worker {
   const CacheAttnParams& p;
   const CachePlan& plan;
   char* lds;  // join_waves: 2 x NT x (E x 4 + 2) x 64 floats; kShared: 2 x (keys, values) tiles
-  int lane, g, c, wave_r, wave_k, key_waves;
+  static constexpr int kWaves = waves_of(kShared);
+  int lane, g, c, chunk, wave_r, wave_k, key_waves;
   int group, rows, row_bytes;
   // byte offsets of the lane's channels in a row (kShared: of LDS)
   uint32_t k_channel[T::kChunks], v_channel[T::H];
@@ -233,8 +228,8 @@ struct Worker {
   uint32_t block_magic;
 
   uint32_t q_hi[NT][T::kChunks][4], q_lo[NT][T::kHalf ? T::kChunks : 1][4];
-  float factor[NT];
-  float m[NT], l[NT];
+  float factor[NT];  // > 0: scores are factor times what the matrix cores give, to the base 2
+  float m[NT], l[NT];  // m: without the factor until the walk ends
   v4f o[NT][T::E];
   v4u k[T::kKeyTiles][T::kChunks];
   uint32_t v[T::kLane][T::H][T::kWords];
@@ -244,6 +239,9 @@ struct Worker {
     lane = threadIdx.x & 63;
     g = lane >> 4;
     c = lane & 15;
+    // Row r of V^T's tiles is channel chunk(r): r with its two base-4 digits exchanged, so that an output
+    // row's four lanes hold neighbouring chunks and store whole lines together.
+    chunk = (c & 3) * 4 + (c >> 2);
     const int wave = uniform(threadIdx.x >> 6);
     wave_r = wave % plan.row_waves;
     wave_k = wave / plan.row_waves;
@@ -261,7 +259,7 @@ struct Worker {
     }
 #pragma unroll
     for (int h = 0; h < T::H; ++h) {
-      const int byte = (h * 16 + c) * T::W * T::kBytes;
+      const int byte = (h * 16 + chunk) * T::W * T::kBytes;
       v_channel[h] = kShared || byte < row_bytes ? byte : kNoChannel;
     }
   }
@@ -297,50 +295,50 @@ struct Worker {
     }
   }
 
+  // Rows that are not there repeat row 0, channels behind dhead the first ones (their keys are zeros):
+  // nothing of them is stored, and all loads go out together.
   __device__ __forceinline__ void load_queries() {
+    const float sign = p.scale < 0.f ? -1.f : 1.f, size = fabsf(p.scale) * kLog2e;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + n * 16 + c;
       const float* q = p.q + row_at(row < rows ? row : 0);
-      if constexpr (T::kHalf) {
-        float x[T::kChunks][8];
-        float most = 0.f;
+      constexpr int kFloats = T::kHalf ? 8 : 4;
+      float x[T::kChunks][kFloats];
 #pragma unroll
-        for (int s = 0; s < T::kChunks; ++s) {
-          const int d = s * 32 + g * 8;
-          const bool there = row < rows && d < p.dhead;
+      for (int s = 0; s < T::kChunks; ++s) {
+        const int d = (s * 4 + g) * kFloats;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {  // (loads without a branch: all are requested before the first is used)
-            const v4f y = *reinterpret_cast<const v4f*>(q + (d < p.dhead ? d : 0) + 4 * i);
+        for (int i = 0; i < kFloats; i += 4) {
+          const v4f y = *reinterpret_cast<const v4f*>(q + (d < p.dhead ? d : 0) + i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[s][4 * i + j] = there ? y[j] : 0.f;
-          }
+          for (int j = 0; j < 4; ++j) x[s][i + j] = y[j];
         }
+      }
+      float f = size;
+      if constexpr (T::kHalf) {
+        float most = 1.17549435e-38f;
 #pragma unroll
         for (int s = 0; s < T::kChunks; ++s)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[s][j]));
+          for (int j = 0; j < kFloats; ++j) most = fmaxf(most, fabsf(x[s][j]));
         // to [1, 2) by a power of two, which the factor takes back: float16 has no room for less or more
-        const int power = ilogbf(fmaxf(rows_max(most), 1.17549435e-38f));
-        const int shift = power > 126 ? 126 : power;
-        factor[n] = p.scale * kLog2e * ldexpf(1.f, shift);
-        const float down = ldexpf(1.f, -shift);
+        const uint32_t exponent = __float_as_uint(rows_max(most)) >> 23;  // 1 .. 255
+        const uint32_t e = exponent < 253 ? exponent : 253;
+        f *= __uint_as_float(e << 23);
+        const float down = sign * __uint_as_float((254 - e) << 23);
 #pragma unroll
         for (int s = 0; s < T::kChunks; ++s)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, q_hi[n][s][j], q_lo[n][s][j]);
       } else {
-        factor[n] = p.scale * kLog2e;
 #pragma unroll
-        for (int s = 0; s < T::kChunks; ++s) {
-          const int d = s * 16 + g * 4;
-          const v4f y = *reinterpret_cast<const v4f*>(q + (d < p.dhead ? d : 0));
-          const bool there = row < rows && d < p.dhead;
+        for (int s = 0; s < T::kChunks; ++s)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = there ? __float_as_uint(y[j]) : 0u;
-        }
+          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = __float_as_uint(x[s][j] * sign);
       }
+      factor[n] = f < 1.17549435e-38f ? 1.17549435e-38f : f;  // (above zero: -inf times it stays -inf)
     }
   }
 
@@ -397,19 +395,20 @@ struct Worker {
   // number of the lane that will read it as its A row, which puts the 16 rows that lanes read
   // together on all banks - is made by what a lane asks for.
   __device__ __forceinline__ void stage(int t, int buffer) {
-    constexpr int kLoads = T::kTileBytes / (kThreads * 16);
-    int thread = threadIdx.x;
-    rare(thread);  // (the offsets are made again per tile: kept, they would cost the registers of a row tile)
-    char* to = lds + buffer * 2 * T::kTileBytes + uniform(threadIdx.x >> 6) * 1024;
+    char* to = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
+    int at = lane;
+    rare(at);  // (the offsets are made again per tile: kept, they would cost the registers of a row tile)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * kThreads + thread, row = at / T::kRowChunks, unit = at % T::kRowChunks;
+    for (int i = 0; i < 4; ++i) {
+      const int piece = wave_r + i * plan.row_waves;  // of 1 KB
+      if (piece >= T::kTileBytes / 1024) break;
+      const int row = (piece * 64 + at) / T::kRowChunks, unit = at % T::kRowChunks;
       const int reader = T::kHalf ? (row & 3) | (row >> 3 & 3) << 2 : row & 15;
       const int k_byte = (unit ^ (reader % T::kRowChunks)) * 16, v_byte = unit * 16;
       const uint32_t from = static_cast<uint32_t>(t + row) * static_cast<uint32_t>(row_bytes);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(k_rsrc, (lds_void*)(to + i * kThreads * 16), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(k_rsrc, (lds_void*)(to + piece * 1024), 16,
                                                from + (k_byte < row_bytes ? k_byte : kNoChannel), 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(v_rsrc, (lds_void*)(to + T::kTileBytes + i * kThreads * 16), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(v_rsrc, (lds_void*)(to + T::kTileBytes + piece * 1024), 16,
                                                from + (v_byte < row_bytes ? v_byte : kNoChannel), 0, 0, 0);
     }
   }
@@ -492,31 +491,43 @@ struct Worker {
   __device__ __forceinline__ void advance(int step, int next, const char* tile = nullptr, int first = 0) {
     if constexpr (kShared) read_keys(tile, first);
     float s[NT][T::kLane];
+    {
+      v4f acc[NT][T::kKeyTiles];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < T::kKeyTiles; ++i) {
-        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < T::kKeyTiles; ++i) acc[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+      // (independent products follow each other: a product waits for the one that it adds to)
+#pragma unroll
+      for (int x = 0; x < T::kChunks; ++x)
         if constexpr (T::kHalf) {
 #pragma unroll
-          for (int x = 0; x < T::kChunks; ++x) {
-            acc = Mfma<kType>::mul(k[i][x], v4u{q_hi[n][x][0], q_hi[n][x][1], q_hi[n][x][2], q_hi[n][x][3]}, acc);
-            acc = Mfma<kType>::mul(k[i][x], v4u{q_lo[n][x][0], q_lo[n][x][1], q_lo[n][x][2], q_lo[n][x][3]}, acc);
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < T::kKeyTiles; ++i)
+              acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{q_hi[n][x][0], q_hi[n][x][1], q_hi[n][x][2], q_hi[n][x][3]},
+                                           acc[n][i]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < T::kKeyTiles; ++i)
+              acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{q_lo[n][x][0], q_lo[n][x][1], q_lo[n][x][2], q_lo[n][x][3]},
+                                           acc[n][i]);
         } else {
 #pragma unroll
-          for (int x = 0; x < T::kChunks; ++x)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][x][j]), __uint_as_float(q_hi[n][x][j]),
-                                                         acc, 0, 0, 0);
+            for (int n = 0; n < NT; ++n)
+              acc[n][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[0][x][j]),
+                                                               __uint_as_float(q_hi[n][x][j]), acc[n][0], 0, 0, 0);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][i * 4 + j] = acc[j] * factor[n];
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < T::kLane; ++j) s[n][j] = acc[n][j / 4][j % 4];
     }
-    if constexpr (kShared) read_values(tile + T::kTileBytes, first);
-    else load_keys(next);
+    if constexpr (!kShared) load_keys(next);
+    else if constexpr (kPlain) read_values(tile + T::kTileBytes, first);
 
     uint32_t hidden[NT];  // bit j: the row does not see the lane's position j
     bool full = true;
@@ -547,7 +558,8 @@ struct Worker {
                       ((b * p.heads_kv + hkv) * rows + row) * plan.score_pitch + step + g * T::kLane;
 #pragma unroll
           for (int j = 0; j < T::kLane; j += 4)
-            *reinterpret_cast<v4f*>(to + j) = v4f{s[n][j], s[n][j + 1], s[n][j + 2], s[n][j + 3]};
+            *reinterpret_cast<v4f*>(to + j) =
+                v4f{s[n][j], s[n][j + 1], s[n][j + 2], s[n][j + 3]} * factor[n];
         }
       }
     }
@@ -558,21 +570,25 @@ struct Worker {
 #pragma unroll
       for (int j = 1; j < T::kLane; ++j) most = fmaxf(most, s[n][j]);
       most = fmaxf(m[n], rows_max(most));
-      const float base = finite_base(most);
       if (__any(most > m[n])) {
-        const float keep = shift_of(m[n], base);
+        const float keep = __builtin_amdgcn_exp2f((m[n] - finite_base(most)) * factor[n]);
         l[n] *= keep;
 #pragma unroll
         for (int e = 0; e < T::E; ++e) o[n][e] *= keep;
         m[n] = most;
       }
+      const float base = finite_base(most) * factor[n];
 #pragma unroll
       for (int j = 0; j < T::kLane; ++j) {
-        s[n][j] = __builtin_amdgcn_exp2f(s[n][j] - base);
+        s[n][j] = __builtin_amdgcn_exp2f(fmaf(s[n][j], factor[n], -base));
         l[n] += s[n][j];
       }
     }
 
+    if constexpr (kShared && !kPlain) {
+      __builtin_amdgcn_sched_barrier(0);  // (not before the keys' registers are free)
+      read_values(tile + T::kTileBytes, first);
+    }
     bool apart = false;
     if constexpr (kView == CacheView::kTree && !kPlain) {
       apart = !full && !__all(values_finite());
@@ -645,7 +661,7 @@ struct Worker {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // channels behind dhead read as zeros or as other channels: they are not stored
-          const uint32_t byte = row + (h * 16 + g * 4 + i) * T::W * T::kBytes;
+          const uint32_t byte = row + (h * 16 + i * 4 + g) * T::W * T::kBytes;
           v2u y[T::kWords / 2];
 #pragma unroll
           for (int w = 0; w < T::kWords / 2; ++w)
@@ -670,17 +686,18 @@ struct Worker {
     }
   }
 
-  // the tile of round r, once it has arrived; the next one is requested before it is used
+  // the wave's tile of round r, once it has arrived; the next one is requested before it is used
   template <bool kPlain>
   __device__ __forceinline__ void advance_tile(int r, int r0, int r1) {
     // this tile has arrived and the other one is read: no later request may still be under way here
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (r + 1 < r1) stage((r + 1) * T::kTileKeys, (r + 1 - r0) & 1);
-    const char* tile = lds + ((r - r0) & 1) * 2 * T::kTileBytes;
+    const int t = (r * key_waves + wave_k) * T::kTileKeys, buffer = (r - r0) & 1;
+    if (r + 1 < r1) stage(t + key_waves * T::kTileKeys, buffer ^ 1);
+    const char* tile = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
 #pragma unroll 1
     for (int i = 0; i < T::kTileKeys; i += T::kStep)
-      if (kPlain || r * T::kTileKeys + i < end) advance<kPlain>(r * T::kTileKeys + i, 0, tile, i);
+      if (kPlain || t + i < end) advance<kPlain>(t + i, 0, tile, i);
   }
 
   // rounds r0 .. r1 - 1 of the unit: those over committed positions alone first (the loop that counts
@@ -688,8 +705,8 @@ struct Worker {
   __device__ __forceinline__ void walk(int r0, int r1) {
     if constexpr (kShared) {
       __syncthreads();  // nobody reads the tiles of the unit before
-      stage(r0 * T::kTileKeys, 0);
-      const int plain = len / T::kTileKeys;
+      stage((r0 * key_waves + wave_k) * T::kTileKeys, 0);
+      const int plain = len / plan.round_keys;
       int r = r0;
 #pragma unroll 1
       for (; r < r1 && r < plain; ++r) advance_tile<true>(r, r0, r1);
@@ -719,7 +736,10 @@ struct Worker {
       }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) l[n] = rows_sum(l[n]);
+    for (int n = 0; n < NT; ++n) {
+      l[n] = rows_sum(l[n]);
+      if (m[n] != -INFINITY) m[n] *= factor[n];
+    }
   }
 
   // waves that took other positions of the same rows hand theirs to the first
@@ -761,7 +781,7 @@ struct Worker {
 
   // the unit's outputs, or a part's (m, l, o)
   __device__ __forceinline__ void finish(bool complete, int64_t part) {
-    if (!kShared && key_waves > 1) join_waves();
+    if (key_waves > 1) join_waves();
     if (wave_k != 0) return;
     float* scratch = static_cast<float*>(p.scratch);
 #pragma unroll
@@ -787,7 +807,7 @@ struct Worker {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int w = 0; w < T::W; w += 4) {
-            const int d = (h * 16 + g * 4 + i) * T::W + w;
+            const int d = (h * 16 + i * 4 + g) * T::W + w;
             v4f x;
 #pragma unroll
             for (int y = 0; y < 4; ++y) x[y] = l[n] == 0.f ? 0.f : o[n][h * T::W + w + y][i] * by;
@@ -797,67 +817,73 @@ struct Worker {
   }
 };
 
-constexpr int waves_per_simd(int dp, int nt, bool shared) {
-  return dp == 256 || (dp * nt == 256 && !shared) ? 1 : 2;
-}
+constexpr int waves_per_simd(int dp) { return dp == 256 ? 1 : 2; }
 
 template <int kType, int DP, int NT, CacheView kView, bool kShared>
-__global__ __launch_bounds__(kThreads, waves_per_simd(DP, NT, kShared))
+__global__ __launch_bounds__(64 * waves_of(kShared), waves_per_simd(DP))
 void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   Worker<kType, DP, NT, kView, kShared> worker(p, plan, lds);
-  const int units = static_cast<int>(p.heads_kv) * plan.row_groups;
+  const uint32_t units = static_cast<uint32_t>(p.heads_kv) * plan.row_groups;
   Line line{0, 0, 1, 0};
-  int64_t b = 0, before = 0, x, x1;  // entry, the round of the line that it begins at, the stretch
+  int64_t b = 0;
+  uint32_t before = 0, x, x1;  // the round of the line that entry b begins at, the workgroup's stretch
   if (plan.whole) {  // a line of the one entry
     b = blockIdx.x / units;
-    const int n = uniform(rounds_of(p, plan, b));
-    x = static_cast<int64_t>(blockIdx.x % units) * n;
+    const uint32_t n = uniform(rounds_of(p, plan, b));
+    x = blockIdx.x % units * n;
     x1 = x + n;
   } else {
-    line = make_line(p, plan);
+    const int lane = threadIdx.x & 63;
+    auto rounds = [&](int64_t entry) {
+      return entry < p.batch ? static_cast<uint32_t>(rounds_of(p, plan, entry)) * units : 0u;
+    };
+    uint32_t upto = 0, mine = 0;
+    for (int64_t b0 = 0; b0 < p.batch; b0 += 64) {
+      mine = rounds(b0 + lane);
+      upto = wave_scan(mine);
+      line.total += __builtin_amdgcn_readlane(upto, 63);
+    }
+    const uint32_t groups = line.total / plan.min_rounds;
+    line.groups = groups < 1 ? 1 : (groups > static_cast<uint32_t>(plan.grid) ? plan.grid : groups);
+    line.each = line.total / line.groups;
+    line.longer = line.total - line.each * line.groups;
     if (blockIdx.x >= line.groups) return;
     x = line.start(blockIdx.x);
     x1 = line.start(blockIdx.x + 1);
-    // the entry that x lies in: 64 entries at a time
+    // the entry that x lies in
     for (;; b += 64) {
-      const int lane = threadIdx.x & 63;
-      const int64_t mine = b + lane < p.batch ? static_cast<int64_t>(rounds_of(p, plan, b + lane)) * units : 0;
-      int64_t upto = mine;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(static_cast<long long>(upto), o, 64);
-        if (lane >= o) upto += y;
+      if (p.batch > 64) {
+        mine = rounds(b + lane);
+        upto = wave_scan(mine);
       }
       const uint64_t behind = __ballot(before + upto > x);
       if (behind) {
         const int at = __builtin_ctzll(behind);
-        before += __shfl(static_cast<long long>(upto - mine), at);
+        before += __builtin_amdgcn_readlane(upto - mine, at);
         b += at;
         break;
       }
-      before += __shfl(static_cast<long long>(upto), 63);
+      before += __builtin_amdgcn_readlane(upto, 63);
     }
-    b = uniform64(b);
-    before = uniform64(before);
   }
-  const int64_t x0 = x;
+  const uint32_t x0 = x;
 #pragma unroll 1
   while (x < x1) {
-    const int n = uniform(rounds_of(p, plan, b));
-    const int64_t within = x - before;
-    const int unit = static_cast<int>(divide(within, n)), r0 = static_cast<int>(within - static_cast<int64_t>(unit) * n);
-    const int r1 = static_cast<int>(x1 - x < n - r0 ? r0 + (x1 - x) : n);
+    const uint32_t n = uniform(rounds_of(p, plan, b));
+    const uint32_t unit = (x - before) / n, r0 = x - before - unit * n;
+    const uint32_t r1 = x1 - x < n - r0 ? r0 + (x1 - x) : n;
     worker.begin(b, unit);
     worker.walk(r0, r1);
     // a part that begins the workgroup's stretch is its first, any other its last
     const int slot = blockIdx.x * 2 + (x == x0 ? 0 : 1);
     if (!plan.whole && r0 == 0 && threadIdx.x == 0) {
-      const int count = static_cast<int>(line.holder(x + n - 1)) - static_cast<int>(blockIdx.x) + 1;
+      const int count = static_cast<int>(line.holder(x + n - 1) - blockIdx.x) + 1;
       reinterpret_cast<int2*>(static_cast<float*>(p.scratch) + plan.records)[b * units + unit] = int2{slot, count};
     }
     worker.finish(r0 == 0 && r1 == n, slot);
     x += r1 - r0;
-    if (x == before + static_cast<int64_t>(n) * units) {
+    if (x == before + n * units) {
       before = x;
       ++b;
     }
@@ -884,7 +910,7 @@ __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
   constexpr int kAhead = 4;  // parts requested together
   const int lane = threadIdx.x & 63;
   const int group = static_cast<int>(p.heads / p.heads_kv), rows = static_cast<int>(p.tokens) * group;
-  const int64_t at = blockIdx.x * static_cast<int64_t>(kWaves) + uniform(threadIdx.x >> 6);
+  const int64_t at = blockIdx.x * static_cast<int64_t>(kThreads / 64) + uniform(threadIdx.x >> 6);
   const int64_t unit = at / plan.unit_rows, head = unit / plan.row_groups;
   if (head >= p.batch * p.heads_kv) return;
   const int local = static_cast<int>(at - unit * plan.unit_rows);
@@ -994,15 +1020,17 @@ CachePlan make_plan(const CacheAttnParams& p) {
   CachePlan plan;
   const int64_t rows = p.tokens * (p.heads / p.heads_kv);
   const int dp = padded_head(p.dhead), element = p.kv_dtype == kF32 ? 4 : 2;
-  // Few rows: every wave takes all of them and its own positions. From 33 on: a wave has its own 16 or
-  // 32, and the positions are shared through LDS.
-  plan.shared = p.view == CacheView::kTree && rows > 32;
-  plan.tiles = p.view != CacheView::kTree || rows <= 16 || dp == 256 || (plan.shared && rows <= 64) ? 1 : 2;
-  plan.row_waves = plan.shared || rows > 32 * plan.tiles ? 4 : (rows > 16 * plan.tiles ? 2 : 1);
+  // Few rows: every wave loads for itself. From 33 on, heads of up to 128: tiles in LDS, which four or
+  // eight waves with rows of their own share (16 each up to 64 rows, 32 beyond).
+  plan.shared = p.view == CacheView::kTree && rows > 32 && dp <= 128;
+  const int waves = waves_of(plan.shared);
+  plan.tiles = plan.shared && rows > 64 ? 2 : 1;
+  plan.row_waves = plan.shared ? 4 : 1;
+  while (plan.row_waves < waves && plan.row_waves * 16 * plan.tiles < rows) plan.row_waves *= 2;
   plan.unit_rows = 16 * plan.tiles * plan.row_waves;
   plan.row_groups = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
-  plan.round_keys = plan.shared ? 16384 / (dp * element) : (element == 4 ? 16 : 32) * (kWaves / plan.row_waves);
-  plan.grid = 512;
+  plan.round_keys = (plan.shared ? 16384 / (dp * element) : element == 4 ? 16 : 32) * (waves / plan.row_waves);
+  plan.grid = plan.shared ? 256 : 512;
   plan.min_rounds = 4;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
@@ -1022,7 +1050,7 @@ CachePlan make_plan(const CacheAttnParams& p) {
     plan.scores = plan.stats + up(p.batch * p.heads * 2);
     plan.total = plan.scores + p.batch * p.heads * plan.score_pitch;
   }
-  plan.join_groups = plan.whole ? 0 : static_cast<int>((units * plan.unit_rows + kWaves - 1) / kWaves);
+  plan.join_groups = plan.whole ? 0 : static_cast<int>((units * plan.unit_rows + kThreads / 64 - 1) / (kThreads / 64));
   plan.weight_tiles =
       p.weights ? static_cast<int>((p.t_max + kThreads * kWeightSteps - 1) / (kThreads * kWeightSteps)) : 0;
   return plan;
@@ -1031,11 +1059,24 @@ CachePlan make_plan(const CacheAttnParams& p) {
 template <int kType, int DP, int NT, CacheView kView, bool kShared = false>
 void launch_tiles(const CacheAttnParams& p, const CachePlan& plan, hipStream_t stream) {
   using T = Tile<kType, DP, NT>;
+  constexpr int waves = waves_of(kShared);
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  const size_t lds = kShared ? 4 * T::kTileBytes
-                             : plan.row_waves < kWaves ? sizeof(float) * (kWaves / 2) * NT * (T::E * 4 + 2) * 64 : 0;
-  hipLaunchKernelGGL((cache_attention_kernel<kType, DP, NT, kView, kShared>),
-                     dim3(static_cast<unsigned>(plan.whole ? units : plan.grid)), dim3(kThreads), lds, stream, p, plan);
+  const int key_waves = waves / plan.row_waves;
+  const size_t join = key_waves > 1 ? sizeof(float) * (waves / 2) * NT * (T::E * 4 + 2) * 64 : 0;
+  const size_t lds = kShared ? std::max<size_t>(join, 4 * T::kTileBytes * key_waves) : join;
+  const auto kernel = cache_attention_kernel<kType, DP, NT, kView, kShared>;
+  if constexpr (kShared) {  // more than 64 KiB of dynamic LDS has to be opted into once per device
+    static std::atomic<bool> configured[64];
+    int device = 0;
+    CT2X_HIP_CHECK(hipGetDevice(&device));
+    if (!configured[device & 63].load(std::memory_order_acquire)) {
+      CT2X_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+      configured[device & 63].store(true, std::memory_order_release);
+    }
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.whole ? units : plan.grid)), dim3(64 * waves), lds, stream,
+                     p, plan);
 }
 
 template <int kType, int DP>
@@ -1043,12 +1084,10 @@ void launch_head(const CacheAttnParams& p, const CachePlan& plan, hipStream_t st
   if (p.view == CacheView::kDense) return launch_tiles<kType, DP, 1, CacheView::kDense>(p, plan, stream);
   if (p.view == CacheView::kBlocks) return launch_tiles<kType, DP, 1, CacheView::kBlocks>(p, plan, stream);
   if constexpr (DP < 256) {
-    if (plan.tiles == 2)
-      return plan.shared ? launch_tiles<kType, DP, 2, CacheView::kTree, true>(p, plan, stream)
-                         : launch_tiles<kType, DP, 2, CacheView::kTree>(p, plan, stream);
+    if (plan.shared && plan.tiles == 2) return launch_tiles<kType, DP, 2, CacheView::kTree, true>(p, plan, stream);
+    if (plan.shared) return launch_tiles<kType, DP, 1, CacheView::kTree, true>(p, plan, stream);
   }
-  if (plan.shared) launch_tiles<kType, DP, 1, CacheView::kTree, true>(p, plan, stream);
-  else launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
+  launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
 }
 
 template <int kType>
