@@ -243,6 +243,9 @@ struct Worker {
     // row's four lanes hold neighbouring chunks and store whole lines together.
     chunk = (c & 3) * 4 + (c >> 2);
     const int wave = uniform(threadIdx.x >> 6);
+    // Two waves of a SIMD that run the same code in step want the matrix cores at the same time and
+    // leave them idle at the same time; the first one's priority keeps them apart.
+    if (kShared && wave < kWaves / 2) __builtin_amdgcn_s_setprio(1);
     wave_r = wave % plan.row_waves;
     wave_k = wave / plan.row_waves;
     key_waves = kWaves / plan.row_waves;
@@ -465,6 +468,12 @@ struct Worker {
     return kAll & ~(old | seen);
   }
 
+  __device__ __forceinline__ static bool finite_word(uint32_t x) {
+    if constexpr (kType == kF32) return (x & 0x7f800000u) != 0x7f800000u;
+    constexpr uint32_t e = kType == kF16 ? 0x7c00u : 0x7f80u;
+    return (x & e) != e && (x >> 16 & e) != e;
+  }
+
   __device__ __forceinline__ bool values_finite() const {
     bool fine = true;
 #pragma unroll
@@ -472,22 +481,14 @@ struct Worker {
 #pragma unroll
       for (int h = 0; h < T::H; ++h)
 #pragma unroll
-        for (int w = 0; w < T::kWords; ++w) {
-          const uint32_t x = v[j][h][w];
-          if constexpr (kType == kF32) {
-            fine &= (x & 0x7f800000u) != 0x7f800000u;
-          } else {
-            constexpr uint32_t e = kType == kF16 ? 0x7c00u : 0x7f80u;
-            fine &= (x & e) != e && (x >> 16 & e) != e;
-          }
-        }
+        for (int w = 0; w < T::kWords; ++w) fine &= finite_word(v[j][h][w]);
     return fine;
   }
 
   // one step over positions step .. step + kStep - 1, whose keys and values are in registers or on
-  // their way; `next` is loaded as their registers come free (kShared: they are in `tile`). kPlain: all
-  // positions are committed ones, every row sees them.
-  template <bool kPlain>
+  // their way; `next` is loaded as their registers come free (kShared: they are in `tile`). kApart: a
+  // drafted position among them holds values that are not finite.
+  template <bool kApart>
   __device__ __forceinline__ void advance(int step, int next, const char* tile = nullptr, int first = 0) {
     if constexpr (kShared) read_keys(tile, first);
     float s[NT][T::kLane];
@@ -527,25 +528,21 @@ struct Worker {
         for (int j = 0; j < T::kLane; ++j) s[n][j] = acc[n][j / 4][j % 4];
     }
     if constexpr (!kShared) load_keys(next);
-    else if constexpr (kPlain) read_values(tile + T::kTileBytes, first);
+    else if constexpr (!kApart) read_values(tile + T::kTileBytes, first);
 
     uint32_t hidden[NT];  // bit j: the row does not see the lane's position j
-    bool full = true;
-    if constexpr (!kPlain) {
-      const int at = position(step + g * T::kLane);
-      full = __all(at >= 0 && at + T::kLane <= len);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) hidden[n] = 0u;
-      if (!full) {
+    for (int n = 0; n < NT; ++n) hidden[n] = 0u;
+    const int at = position(step + g * T::kLane);
+    if (kView == CacheView::kBlocks ? !__all(at >= 0 && at + T::kLane <= len) : step + T::kStep > len) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          int row = row0 + n * 16 + c;
-          rare(row);
-          hidden[n] = hidden_from(row, at);
+      for (int n = 0; n < NT; ++n) {
+        int row = row0 + n * 16 + c;
+        rare(row);
+        hidden[n] = hidden_from(row, at);
 #pragma unroll
-          for (int j = 0; j < T::kLane; ++j)
-            if (hidden[n] >> j & 1) s[n][j] = -INFINITY;
-        }
+        for (int j = 0; j < T::kLane; ++j)
+          if (hidden[n] >> j & 1) s[n][j] = -INFINITY;
       }
     }
     if (kView == CacheView::kDense && p.weights) {
@@ -585,16 +582,8 @@ struct Worker {
       }
     }
 
-    if constexpr (kShared && !kPlain) {
-      __builtin_amdgcn_sched_barrier(0);  // (not before the keys' registers are free)
-      read_values(tile + T::kTileBytes, first);
-    }
-    bool apart = false;
-    if constexpr (kView == CacheView::kTree && !kPlain) {
-      apart = !full && !__all(values_finite());
-      if (apart) add_values_apart(step, s, hidden);
-    }
-    if (!apart) add_values(s);
+    if constexpr (kApart) add_values_apart(step, s, hidden);
+    else add_values(s);
     if constexpr (!kShared) load_values(next);
   }
 
@@ -686,52 +675,54 @@ struct Worker {
     }
   }
 
-  // the wave's tile of round r, once it has arrived; the next one is requested before it is used
-  template <bool kPlain>
-  __device__ __forceinline__ void advance_tile(int r, int r0, int r1) {
-    // this tile has arrived and the other one is read: no later request may still be under way here
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    const int t = (r * key_waves + wave_k) * T::kTileKeys, buffer = (r - r0) & 1;
-    if (r + 1 < r1) stage(t + key_waves * T::kTileKeys, buffer ^ 1);
-    const char* tile = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
-#pragma unroll 1
-    for (int i = 0; i < T::kTileKeys; i += T::kStep)
-      if (kPlain || t + i < end) advance<kPlain>(t + i, 0, tile, i);
+  // whether a tile's values are all finite
+  __device__ __forceinline__ bool tile_finite(const char* tile) const {
+    bool fine = true;
+#pragma unroll 2
+    for (int i = lane * 16; i < T::kTileBytes; i += 1024) {
+      const v4u x = *reinterpret_cast<const v4u*>(tile + i);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) fine &= finite_word(x[w]);
+    }
+    return __all(fine);
   }
 
-  // rounds r0 .. r1 - 1 of the unit: those over committed positions alone first (the loop that counts
-  // keeps the masks' code and registers out)
+  // rounds r0 .. r1 - 1 of the unit
   __device__ __forceinline__ void walk(int r0, int r1) {
     if constexpr (kShared) {
       __syncthreads();  // nobody reads the tiles of the unit before
       stage((r0 * key_waves + wave_k) * T::kTileKeys, 0);
-      const int plain = len / plan.round_keys;
-      int r = r0;
 #pragma unroll 1
-      for (; r < r1 && r < plain; ++r) advance_tile<true>(r, r0, r1);
+      for (int r = r0; r < r1; ++r) {
+        // this tile has arrived and the other one is read: no later request may still be under way here
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        const int t = (r * key_waves + wave_k) * T::kTileKeys, buffer = (r - r0) & 1;
+        if (r + 1 < r1) stage(t + key_waves * T::kTileKeys, buffer ^ 1);
+        const char* tile = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
+        if (t + T::kTileKeys > len && !tile_finite(tile + T::kTileBytes)) {
 #pragma unroll 1
-      for (; r < r1; ++r) advance_tile<false>(r, r0, r1);
+          for (int i = 0; i < T::kTileKeys; i += T::kStep)
+            if (t + i < end) advance<true>(t + i, 0, tile, i);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < T::kTileKeys; i += T::kStep)
+            if (t + i < end) advance<false>(t + i, 0, tile, i);
+        }
+      }
     } else {
       auto first = [&](int r) {
         const int t = r * plan.round_keys + wave_k * T::kStep;
         return r < r1 && t < end ? t : -1;
       };
-      int step = first(r0), r = r0;
+      int step = first(r0);
       load_keys(step);
       load_values(step);
-      if constexpr (kView != CacheView::kBlocks) {
 #pragma unroll 1
-        for (; step >= 0 && step + T::kStep <= len; ++r) {
-          const int next = first(r + 1);
-          advance<true>(step, next);
-          step = next;
-        }
-      }
-#pragma unroll 1
-      for (; step >= 0; ++r) {
+      for (int r = r0; step >= 0; ++r) {
         const int next = first(r + 1);
-        advance<false>(step, next);
+        if (kView == CacheView::kTree && step + T::kStep > len && !__all(values_finite())) advance<true>(step, next);
+        else advance<false>(step, next);
         step = next;
       }
     }
