@@ -30,7 +30,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "cache_ops.h"
 #include "device_utils.h"
@@ -117,22 +116,6 @@ struct Line {
     return x < ahead ? x / (each + 1) : longer + (x - ahead) / each;
   }
 };
-
-// sums over the lanes up to each
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  auto moved = [&](auto ctrl, auto rows) {
-    return static_cast<uint32_t>(
-        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  x += moved(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // 1, 2, 4, 8 to the right in a row
-  x += moved(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
-  x += moved(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
-  x += moved(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
-  x += moved(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // the rows before, summed
-  x += moved(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
-  return x;
-}
 
 // ---- the types -------------------------------------------------------------------------------
 
@@ -561,20 +544,32 @@ struct Worker {
       }
     }
 
+    // A maximum that grew by less than kSlack (to the base 2) stays the reference: probabilities up to
+    // 2^kSlack fit every type, and outputs are rescaled seldom.
+    constexpr float kSlack = 8.f;
+    float most[NT];
+    bool grown = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float most = s[n][0];
+      most[n] = s[n][0];
 #pragma unroll
-      for (int j = 1; j < T::kLane; ++j) most = fmaxf(most, s[n][j]);
-      most = fmaxf(m[n], rows_max(most));
-      if (__any(most > m[n])) {
-        const float keep = __builtin_amdgcn_exp2f((m[n] - finite_base(most)) * factor[n]);
+      for (int j = 1; j < T::kLane; ++j) most[n] = fmaxf(most[n], s[n][j]);
+      most[n] = fmaxf(m[n], rows_max(most[n]));
+      grown |= (most[n] - m[n]) * factor[n] > kSlack;
+    }
+    if (__any(grown)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float keep = __builtin_amdgcn_exp2f((m[n] - finite_base(most[n])) * factor[n]);
         l[n] *= keep;
 #pragma unroll
         for (int e = 0; e < T::E; ++e) o[n][e] *= keep;
-        m[n] = most;
+        m[n] = most[n];
       }
-      const float base = finite_base(most) * factor[n];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float base = finite_base(m[n]) * factor[n];
 #pragma unroll
       for (int j = 0; j < T::kLane; ++j) {
         s[n][j] = __builtin_amdgcn_exp2f(fmaf(s[n][j], factor[n], -base));
@@ -956,6 +951,20 @@ __device__ void add_weights(const CacheAttnParams& p, const CachePlan& plan, int
   const int len = committed(p, head / p.heads_kv);
   if (t0 - static_cast<int>(threadIdx.x) >= len) return;
   const float* scratch = static_cast<const float*>(p.scratch);
+  const float* scores = scratch + plan.scores + head * group * plan.score_pitch;
+  float* weights = p.weights + head * p.t_max;
+  // the first heads' scores and the old weights are requested before the statistics are looked for
+  constexpr int kAhead = 4;
+  int t[kWeightSteps];
+  float sum[kWeightSteps], old[kWeightSteps], ahead[kAhead][kWeightSteps];
+#pragma unroll
+  for (int u = 0; u < kWeightSteps; ++u) {
+    t[u] = t0 + u * kThreads < len ? t0 + u * kThreads : 0;
+    sum[u] = 0.f;
+    old[u] = weights[t[u]];
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) ahead[r][u] = scores[(r < group ? r : 0) * plan.score_pitch + t[u]];
+  }
   for (int r = threadIdx.x; r < group; r += kThreads) {
     v2f stats = reinterpret_cast<const v2f*>(scratch + plan.stats)[head * group + r];
     if (!plan.whole) {
@@ -964,8 +973,10 @@ __device__ void add_weights(const CacheAttnParams& p, const CachePlan& plan, int
         const int local = r % plan.unit_rows;
         const v2f* ml = reinterpret_cast<const v2f*>(scratch + plan.parts_ml);
         float most = -INFINITY, total = 0.f;
+#pragma unroll 4
         for (int i = 0; i < parts.count; ++i) most = fmaxf(most, ml[parts.row(plan, i, local)][0]);
         const float base = finite_base(most);
+#pragma unroll 4
         for (int i = 0; i < parts.count; ++i) {
           const v2f part = ml[parts.row(plan, i, local)];
           total += part[1] * shift_of(part[0], base);
@@ -976,26 +987,24 @@ __device__ void add_weights(const CacheAttnParams& p, const CachePlan& plan, int
     stats_s[r] = stats;
   }
   __syncthreads();
-  const float* scores = scratch + plan.scores + head * group * plan.score_pitch;
-  float* weights = p.weights + head * p.t_max;
-  float sum[kWeightSteps], old[kWeightSteps];
-#pragma unroll
-  for (int u = 0; u < kWeightSteps; ++u) {
-    sum[u] = 0.f;
-    old[u] = t0 + u * kThreads < len ? weights[t0 + u * kThreads] : 0.f;
-  }
-#pragma unroll 2
-  for (int r = 0; r < group; ++r) {
+  auto add = [&](int r, const float (&score)[kWeightSteps]) {
     const v2f stats = stats_s[r];
 #pragma unroll
-    for (int u = 0; u < kWeightSteps; ++u) {
-      const int t = t0 + u * kThreads < len ? t0 + u * kThreads : 0;
-      sum[u] += __builtin_amdgcn_exp2f(scores[r * plan.score_pitch + t] - stats[0]) * stats[1];
-    }
+    for (int u = 0; u < kWeightSteps; ++u) sum[u] += __builtin_amdgcn_exp2f(score[u] - stats[0]) * stats[1];
+  };
+#pragma unroll
+  for (int r = 0; r < kAhead; ++r)
+    if (r < group) add(r, ahead[r]);
+#pragma unroll 2
+  for (int r = kAhead; r < group; ++r) {
+    float score[kWeightSteps];
+#pragma unroll
+    for (int u = 0; u < kWeightSteps; ++u) score[u] = scores[r * plan.score_pitch + t[u]];
+    add(r, score);
   }
 #pragma unroll
   for (int u = 0; u < kWeightSteps; ++u)
-    if (t0 + u * kThreads < len) weights[t0 + u * kThreads] = old[u] + sum[u];
+    if (t0 + u * kThreads < len) weights[t[u]] = old[u] + sum[u];
 }
 
 __global__ __launch_bounds__(kThreads) void finish_kernel(CacheAttnParams p, CachePlan plan) {
@@ -1022,7 +1031,7 @@ CachePlan make_plan(const CacheAttnParams& p) {
   plan.row_groups = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
   plan.round_keys = (plan.shared ? 16384 / (dp * element) : element == 4 ? 16 : 32) * (waves / plan.row_waves);
   plan.grid = plan.shared ? 256 : 512;
-  plan.min_rounds = 4;
+  plan.min_rounds = 1;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
   plan.whole = walked <= plan.round_keys * 8 || units >= 2048;

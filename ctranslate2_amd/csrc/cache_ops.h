@@ -7,8 +7,25 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace ct2x {
+
+// sums over the lanes up to each
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  auto moved = [&](auto ctrl, auto rows) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x += moved(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // 1, 2, 4, 8 to the right in a row
+  x += moved(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  x += moved(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // the rows before, summed
+  x += moved(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
+  return x;
+}
 
 // What an attention over the cache reads besides the committed positions of an entry.
 enum class CacheView {

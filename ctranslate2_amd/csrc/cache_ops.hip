@@ -43,23 +43,68 @@ __device__ __forceinline__ K wave_and(K x) {
   return x;
 }
 
-// The `want` (>= 1, <= n) best of key(0 .. n): *threshold = the smallest key taken, returns how many
-// of the keys equal to it are taken. All threads of the workgroup call. Bits that all keys share are
-// skipped (a first pass finds them: scores of one layer have their exponent in common, and every key
-// would meet in one bin), and the search ends with the byte whose bin is taken whole.
+// Keys 0 .. n - 1 spread over a workgroup: every wave has a stretch of them, its lanes the positions
+// in turn. The first kKeep of a lane stay in registers, what a longer row has beyond is read again by
+// every pass.
 template <typename K, typename F>
-__device__ int select_threshold(F key, int n, int want, K* threshold) {
-  __shared__ uint32_t histogram[256];
-  __shared__ K both_s[kSelectThreads / 64], none_s[kSelectThreads / 64];
-  __shared__ uint32_t digit_s, above_s, count_s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  K both = ~static_cast<K>(0), none = both;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += kSelectThreads) {
-    const K x = key(i);
-    both &= x;
-    none &= ~x;
+struct Keys {
+  static constexpr int kKeep = 16;
+  F key;
+  int lane, from, to;
+  K kept[kKeep];
+  __device__ __forceinline__ Keys(F key, int n) : key(key) {
+    const int wave = threadIdx.x >> 6, waves = kSelectThreads / 64;
+    const int stretch = ((n + waves - 1) / waves + 63) / 64 * 64;
+    lane = threadIdx.x & 63;
+    from = wave * stretch;
+    to = from + stretch < n ? from + stretch : n;
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      const int i = from + u * 64 + lane;
+      kept[u] = key(i < to ? i : 0);
+    }
   }
+  // visit(i, key(i), whether there is an i), whole waves at a time
+  template <typename G>
+  __device__ __forceinline__ void each(G visit) const {
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      if (from + u * 64 >= to) return;
+      const int i = from + u * 64 + lane;
+      visit(i, kept[u], i < to);
+    }
+    for (int i0 = from + kKeep * 64; i0 < to; i0 += 64 * 4) {
+      K x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 64 + lane;
+        x[u] = key(i < to ? i : 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 64 + lane;
+        visit(i, x[u], i < to);
+      }
+    }
+  }
+};
+
+// The `want` (1 .. n) best: *threshold = the smallest key taken, returns how many of the keys equal to
+// it are taken. All threads of the workgroup call. Bits that all keys share are skipped (a first pass
+// finds them: scores of one layer have their exponent in common, and every key would meet in one bin),
+// and the search ends with the byte whose bin is taken whole.
+template <typename K, typename F>
+__device__ int select_threshold(const Keys<K, F>& keys, int want, K* threshold) {
+  constexpr int kWaves = kSelectThreads / 64;
+  __shared__ uint32_t histogram[256];
+  __shared__ K both_s[kWaves], none_s[kWaves];
+  __shared__ uint32_t digit_s, above_s, count_s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  K both = ~static_cast<K>(0), none = both;
+  keys.each([&](int, K x, bool there) {
+    both &= there ? x : ~static_cast<K>(0);
+    none &= there ? ~x : ~static_cast<K>(0);
+  });
   both = wave_and(both);
   none = wave_and(none);
   if (lane == 0) {
@@ -67,7 +112,8 @@ __device__ int select_threshold(F key, int n, int want, K* threshold) {
     none_s[wave] = none;
   }
   __syncthreads();
-  for (int w = 0; w < waves; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
     both &= both_s[w];
     none &= none_s[w];
   }
@@ -81,31 +127,32 @@ __device__ int select_threshold(F key, int n, int want, K* threshold) {
   K prefix = both & known;
   while (upto > 0) {
     const int bits = upto < 8 ? upto : 8, shift = upto - bits;
-    __syncthreads();
     if (threadIdx.x < 256) histogram[threadIdx.x] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += kSelectThreads) {
-      const K x = key(i);
-      if ((x & known) == prefix) atomicAdd(&histogram[(x >> shift) & ((1u << bits) - 1)], 1u);
-    }
+    keys.each([&](int, K x, bool there) {
+      if (there && (x & known) == prefix)
+        atomicAdd(&histogram[static_cast<uint32_t>(x >> shift) & ((1u << bits) - 1)], 1u);
+    });
     __syncthreads();
     if (wave == 0) {  // lane 0 has the four highest bins
       uint32_t bin[4], sum = 0;
+#pragma unroll
       for (int i = 0; i < 4; ++i) sum += bin[i] = histogram[255 - 4 * lane - i];
-      uint32_t upto_lane = sum;
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(upto_lane, o, 64);
-        if (lane >= o) upto_lane += y;
-      }
+      const uint32_t upto_lane = wave_scan(sum);
       const uint64_t reached = __ballot(upto_lane >= static_cast<uint32_t>(want));
       if (lane == __builtin_ctzll(reached)) {
-        uint32_t above = upto_lane - sum;
-        int i = 0;
-        while (i < 3 && above + bin[i] < static_cast<uint32_t>(want)) above += bin[i++];
-        digit_s = 255 - 4 * lane - i;
+        uint32_t above = upto_lane - sum, taken = bin[0];
+        int digit = 255 - 4 * lane;
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+          if (above + taken < static_cast<uint32_t>(want)) {
+            above += taken;
+            taken = bin[i];
+            digit = 255 - 4 * lane - i;
+          }
+        digit_s = digit;
         above_s = above;
-        count_s = bin[i];
+        count_s = taken;
       }
     }
     __syncthreads();
@@ -113,45 +160,34 @@ __device__ int select_threshold(F key, int n, int want, K* threshold) {
     prefix |= static_cast<K>(digit_s) << shift;
     known |= static_cast<K>((1u << bits) - 1) << shift;
     upto = shift;
-    if (count_s == static_cast<uint32_t>(want)) {
-      // everything with this prefix is taken: nothing below it is, whatever its lower bits. (As a
-      // threshold the prefix itself: it may be no key, then none is equal to it and all are above.)
-      break;
-    }
+    // Everything with this prefix is taken: nothing below it is, whatever its lower bits. (As a
+    // threshold the prefix itself: it may be no key, then none is equal to it and all are above.)
+    if (count_s == static_cast<uint32_t>(want)) break;
   }
   *threshold = prefix;
   return want;
 }
 
-// emit(slot, i) for the i of 0 .. n with key(i) > threshold or among the first `ties` equal to it,
-// slots 0, 1, .. in order of i. Returns how many. All threads of the workgroup call. A wave takes a
-// stretch of positions: it counts, the waves add up, it emits.
+// emit(slot, i) for the i with key(i) > threshold or among the first `ties` equal to it, slots 0, 1, ..
+// in order of i. Returns how many. All threads of the workgroup call: the waves count, add up, emit.
 template <typename K, typename F, typename G>
-__device__ int emit_selected(F key, int n, K threshold, int ties, G emit) {
-  __shared__ int above_w[kSelectThreads / 64], equal_w[kSelectThreads / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int stretch = ((n + waves - 1) / waves + 63) / 64 * 64;
-  const int from = wave * stretch, to = from + stretch < n ? from + stretch : n;
+__device__ int emit_selected(const Keys<K, F>& keys, K threshold, int ties, G emit) {
+  constexpr int kWaves = kSelectThreads / 64;
+  __shared__ int above_w[kWaves], equal_w[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int above = 0, equal = 0;
-  constexpr int kAhead = 4;  // keys requested together
-  for (int i0 = from; i0 < to; i0 += 64 * kAhead) {
-    K x[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * 64 + lane < to ? key(i0 + u * 64 + lane) : 0;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const bool there = i0 + u * 64 + lane < to;
-      above += __popcll(__ballot(there && x[u] > threshold));
-      equal += __popcll(__ballot(there && x[u] == threshold));
-    }
-  }
+  keys.each([&](int, K x, bool there) {
+    above += __popcll(__ballot(there && x > threshold));
+    equal += __popcll(__ballot(there && x == threshold));
+  });
   if (lane == 0) {
     above_w[wave] = above;
     equal_w[wave] = equal;
   }
   __syncthreads();
   int slot = 0, rank = 0, all = 0, all_equal = 0;
-  for (int w = 0; w < waves; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
     if (w < wave) {
       slot += above_w[w];
       rank += equal_w[w];
@@ -161,22 +197,15 @@ __device__ int emit_selected(F key, int n, K threshold, int ties, G emit) {
   }
   slot += rank < ties ? rank : ties;
   const uint64_t below = (1ull << lane) - 1;
-  for (int i0 = from; i0 < to; i0 += 64 * kAhead) {
-    K x[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * 64 + lane < to ? key(i0 + u * 64 + lane) : 0;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * 64 + lane;
-      const bool same = i < to && x[u] == threshold;
-      const uint64_t same_bits = __ballot(same);
-      const bool take = i < to && (x[u] > threshold || (same && rank + __popcll(same_bits & below) < ties));
-      const uint64_t bits = __ballot(take);
-      if (take) emit(slot + __popcll(bits & below), i);
-      slot += __popcll(bits);
-      rank += __popcll(same_bits);
-    }
-  }
+  keys.each([&](int i, K x, bool there) {
+    const bool same = there && x == threshold;
+    const uint64_t same_bits = __ballot(same);
+    const bool take = there && (x > threshold || (same && rank + __popcll(same_bits & below) < ties));
+    const uint64_t bits = __ballot(take);
+    if (take) emit(slot + __popcll(bits & below), i);
+    slot += __popcll(bits);
+    rank += __popcll(same_bits);
+  });
   return all + (all_equal < ties ? all_equal : ties);
 }
 
@@ -192,9 +221,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvict
   if (n > budget && budget > recent) {
     const int old = n - recent;
     auto key = [&](int i) { return order_key(w[i]); };
+    const Keys<uint32_t, decltype(key)> keys(key, old);
     uint32_t threshold;
-    const int ties = select_threshold<uint32_t>(key, old, budget - recent, &threshold);
-    slot = emit_selected<uint32_t>(key, old, threshold, ties, [&](int at, int i) { positions[at] = i; });
+    const int ties = select_threshold(keys, budget - recent, &threshold);
+    slot = emit_selected(keys, threshold, ties, [&](int at, int i) { positions[at] = i; });
   }
   for (int i = slot + threadIdx.x; i < budget; i += blockDim.x) positions[i] = i < kept ? n - kept + i : -1;
 }
@@ -339,18 +369,20 @@ __global__ __launch_bounds__(kThreads) void block_bounds_kernel(CacheBoundsParam
 
 // scores[b, hkv, j] = max over the group's heads of sum_d (q_d >= 0 ? q_d max_d : q_d min_d), NaN where
 // a bound is; float64, since a choice between blocks must not depend on how the sum was ordered. Eight
-// lanes per block, each with every eighth 16 bytes of its channels; the heads' queries wait in LDS as
-// float64. Bound by the reads of the bounds.
+// lanes per block, each with every eighth 16 bytes of its channels, kPair blocks at a time; the heads'
+// queries wait in LDS as float64, split into max(q, 0) and min(q, 0): two products by converted bounds
+// instead of a choice per head. (An infinite bound times the zero half would be NaN: such blocks are
+// summed by the choice.) Bound by the float64 products and the LDS reads about as much as by the bounds.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParams p, int64_t blocks, int walkers) {
-  constexpr int V = 16 / sizeof(T), kHeads = 4;  // heads at a time
-  __shared__ double q_s[kHeads][256];
+  constexpr int V = 16 / sizeof(T), kHeads = 4, kPair = 4;  // heads, blocks at a time
+  __shared__ double2 q_s[kHeads][256];
   const int64_t row = blockIdx.x / walkers;
   const int64_t b = row / p.heads_kv, hkv = row % p.heads_kv;
   const int group = static_cast<int>(p.heads / p.heads_kv), dhead = static_cast<int>(p.dhead);
   const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
   const int count = static_cast<int>((n + p.block - 1) / p.block);
-  const int per = (count + walkers * 32 - 1) / (walkers * 32) * 32, from = static_cast<int>(blockIdx.x % walkers) * per;
+  const int per = (count + walkers * kPair * 32 - 1) / (walkers * kPair * 32) * kPair * 32, from = static_cast<int>(blockIdx.x % walkers) * per;
   const int to = from + per < count ? from + per : count;
   if (from >= to || count <= p.top) return;  // (all blocks are taken: no scores are looked at)
   const int part = threadIdx.x & 7;
@@ -358,39 +390,75 @@ __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParam
   for (int h0 = 0; h0 < group; h0 += kHeads) {
     const int heads = group - h0 < kHeads ? group - h0 : kHeads;
     __syncthreads();
-    for (int i = threadIdx.x; i < kHeads * dhead; i += kThreads)
-      q_s[i / dhead][i % dhead] =
-          i / dhead < heads ? p.q[(b * p.heads + hkv * group + h0) * dhead + i] : 0.;
+    for (int i = threadIdx.x; i < kHeads * dhead; i += kThreads) {
+      const int h = i / dhead;
+      const double q = h < heads ? p.q[(b * p.heads + hkv * group + h0) * dhead + i] : 0.;
+      q_s[h][i - h * dhead] = q >= 0. ? double2{q, 0.} : q < 0. ? double2{0., q} : double2{q, q};
+    }
     __syncthreads();
-    for (int j0 = from; j0 < to; j0 += kThreads / 8) {
-      const int j = j0 + (threadIdx.x >> 3);
-      const T* low = bounds + static_cast<int64_t>(j < to ? j : to - 1) * 2 * dhead;
-      double sum[kHeads] = {0., 0., 0., 0.};
-      bool fine = true;
+    for (int j0 = from; j0 < to; j0 += kPair * kThreads / 8) {
+      const T* low[kPair];
+      double sum[kPair][kHeads] = {};
+      bool fine[kPair], finite = true;
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) {
+        const int j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
+        low[u] = bounds + static_cast<int64_t>(j < to ? j : to - 1) * 2 * dhead;
+        fine[u] = true;
+      }
       for (int d = part * V; d < dhead; d += 8 * V) {
-        float x[V], y[V];
-        unpack<T>(*reinterpret_cast<const int4*>(low + d), x);
-        unpack<T>(*reinterpret_cast<const int4*>(low + dhead + d), y);
+        float x[kPair][V], y[kPair][V];
+#pragma unroll
+        for (int u = 0; u < kPair; ++u) {
+          unpack<T>(*reinterpret_cast<const int4*>(low[u] + d), x[u]);
+          unpack<T>(*reinterpret_cast<const int4*>(low[u] + dhead + d), y[u]);
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          fine &= x[i] == x[i] && y[i] == y[i];
+          double a[kPair], c[kPair];  // (converted once for all heads)
+#pragma unroll
+          for (int u = 0; u < kPair; ++u) {
+            a[u] = x[u][i];
+            c[u] = y[u][i];
+            fine[u] &= !__builtin_isunordered(x[u][i], y[u][i]);
+            finite &= fabsf(x[u][i]) < INFINITY && fabsf(y[u][i]) < INFINITY;
+          }
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
-            const double q = q_s[h][d + i];
-            sum[h] = fma(q, static_cast<double>(q >= 0. ? y[i] : x[i]), sum[h]);
+            const double2 q = q_s[h][d + i];
+#pragma unroll
+            for (int u = 0; u < kPair; ++u) sum[u][h] = fma(q.y, a[u], fma(q.x, c[u], sum[u][h]));
           }
         }
       }
+      if (!__all(finite)) {
 #pragma unroll
-      for (int h = 0; h < kHeads; ++h)
-        for (int o = 1; o < 8; o <<= 1) sum[h] += __shfl_xor(sum[h], o, 64);
-      for (int o = 1; o < 8; o <<= 1) fine &= __shfl_xor(static_cast<int>(fine), o, 64) != 0;
-      if (part == 0 && j < to) {
-        double best = h0 ? p.scores[row * blocks + j] : sum[0];
+        for (int u = 0; u < kPair; ++u)
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) {
+            sum[u][h] = 0.;
+            for (int d = part * V; d < dhead; d += 8 * V)
+              for (int i = d; i < d + V; ++i) {
+                const double q = q_s[h][i].x + q_s[h][i].y;
+                sum[u][h] = fma(q, static_cast<double>(load_float(low[u][q >= 0. ? dhead + i : i])), sum[u][h]);
+              }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) {
+        const int j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
-          if (h < heads && (sum[h] > best || sum[h] != sum[h])) best = sum[h];
-        p.scores[row * blocks + j] = fine ? best : __builtin_nan("");
+          for (int o = 1; o < 8; o <<= 1) sum[u][h] += __shfl_xor(sum[u][h], o, 64);
+        int all = fine[u];
+        for (int o = 1; o < 8; o <<= 1) all &= __shfl_xor(all, o, 64);
+        if (part == 0 && j < to) {
+          double best = h0 ? p.scores[row * blocks + j] : sum[u][0];
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h)
+            if (h < heads && (sum[u][h] > best || sum[u][h] != sum[u][h])) best = sum[u][h];
+          p.scores[row * blocks + j] = all ? best : __builtin_nan("");
+        }
       }
     }
   }
@@ -404,9 +472,10 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(CacheSelec
   int32_t* selected = p.selected + row * p.top;
   if (count > top) {
     auto key = [&](int j) { return j < p.sink || j >= count - p.local ? ~0ull : order_key(scores[j]); };
+    const Keys<uint64_t, decltype(key)> keys(key, count);
     uint64_t threshold;
-    const int ties = select_threshold<uint64_t>(key, count, top, &threshold);
-    emit_selected<uint64_t>(key, count, threshold, ties, [&](int at, int j) { selected[at] = j; });
+    const int ties = select_threshold(keys, top, &threshold);
+    emit_selected(keys, threshold, ties, [&](int at, int j) { selected[at] = j; });
   } else {
     for (int j = threadIdx.x; j < top; j += blockDim.x) selected[j] = j < count ? j : -1;
   }
@@ -431,7 +500,7 @@ void bounds_typed(const CacheBoundsParams& p, int64_t blocks, hipStream_t stream
 template <typename T>
 void scores_typed(const CacheSelectParams& p, int64_t blocks, hipStream_t stream) {
   const int64_t rows = p.batch * p.heads_kv;
-  const int walkers = walkers_for(rows, (blocks + kThreads / 8 - 1) / (kThreads / 8));
+  const int walkers = walkers_for(rows, (blocks + kThreads / 2 - 1) / (kThreads / 2));
   hipLaunchKernelGGL((block_scores_kernel<T>), dim3(static_cast<unsigned>(rows * walkers)), dim3(kThreads), 0, stream,
                      p, blocks, walkers);
 }
