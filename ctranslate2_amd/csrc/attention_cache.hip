@@ -64,7 +64,9 @@ struct CachePlan {
                     // different positions
   int unit_rows;    // rows of a unit
   int row_groups;   // units per (entry, head of the cache)
-  int round_keys;   // positions of a round
+  int round_shift;  // log2 of the positions of a round
+  int group, rows;  // heads of a head of the cache, rows of an entry and head
+  uint32_t block_magic;  // ceil(2^32 / (block / 16)), 0 for blocks of 16
   int grid;         // workgroups at most
   int min_rounds;   // per workgroup
   bool whole;       // one workgroup per unit
@@ -95,13 +97,13 @@ __device__ __forceinline__ int walked(const CacheAttnParams& p, int64_t b) {
   const int n = committed(p, b);
   if (p.view == CacheView::kTree) return n + static_cast<int>(p.tokens);
   if (p.view == CacheView::kDense) return n;
-  const int64_t blocks = (n + p.block - 1) / p.block;
-  return static_cast<int>((blocks < p.top ? blocks : p.top) * p.block);
+  const int block = static_cast<int>(p.block), blocks = (n + block - 1) / block, top = static_cast<int>(p.top);
+  return (blocks < top ? blocks : top) * block;
 }
 
 // at least one: an entry without positions still has outputs to write
 __device__ __forceinline__ int rounds_of(const CacheAttnParams& p, const CachePlan& plan, int64_t b) {
-  const int n = (walked(p, b) + plan.round_keys - 1) / plan.round_keys;
+  const int n = (walked(p, b) + (1 << plan.round_shift) - 1) >> plan.round_shift;
   return n < 1 ? 1 : n;
 }
 
@@ -208,7 +210,6 @@ struct Worker {
   const char *k_base, *v_base;
   __amdgpu_buffer_rsrc_t k_rsrc, v_rsrc;
   const int32_t* selected;
-  uint32_t block_magic;
 
   uint32_t q_hi[NT][T::kChunks][4], q_lo[NT][T::kHalf ? T::kChunks : 1][4];
   float factor[NT];  // > 0: scores are factor times what the matrix cores give, to the base 2
@@ -232,11 +233,9 @@ struct Worker {
     wave_r = wave % plan.row_waves;
     wave_k = wave / plan.row_waves;
     key_waves = kWaves / plan.row_waves;
-    group = static_cast<int>(p.heads / p.heads_kv);
-    rows = static_cast<int>(p.tokens) * group;
+    group = plan.group;
+    rows = plan.rows;
     row_bytes = static_cast<int>(p.dhead) * T::kBytes;
-    if constexpr (kView == CacheView::kBlocks)
-      block_magic = static_cast<uint32_t>(((1ull << 32) + p.block / 16 - 1) / (p.block / 16));
 #pragma unroll
     for (int s = 0; s < T::kChunks; ++s) {
       const int byte = s * 64 + g * 16;
@@ -256,7 +255,8 @@ struct Worker {
     return ((b * p.tokens + i) * p.heads + hkv * group + h) * p.dhead;
   }
 
-  __device__ __forceinline__ void begin(int64_t entry, int unit) {
+  // the unit's rounds r0 .. r1 - 1: their first keys and values are requested before the queries
+  __device__ __forceinline__ void begin(int64_t entry, int unit, int r0, int r1) {
     b = entry;
     hkv = unit / plan.row_groups;
     row0 = (unit % plan.row_groups * plan.row_waves + wave_r) * NT * 16;
@@ -271,6 +271,14 @@ struct Worker {
     k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(k_base), 0, reach, 0x00027000);
     v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(v_base), 0, reach, 0x00027000);
     if constexpr (kView == CacheView::kBlocks) selected = p.selected + uniform64(head * p.top);
+    if constexpr (kShared) {
+      __syncthreads();  // nobody reads the tiles of the unit before
+      stage((r0 * key_waves + wave_k) * T::kTileKeys, 0);
+    } else {
+      const int step = step_of(r0, r1);
+      load_keys(step);
+      load_values(step);
+    }
     load_queries();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -331,11 +339,12 @@ struct Worker {
   // cache position of walked position t (a multiple of 4); negative: none
   __device__ __forceinline__ int position(int t) const {
     if constexpr (kView != CacheView::kBlocks) return t;
-    const uint32_t u = static_cast<uint32_t>(t) >> 4, j = __umulhi(u, block_magic);
-    const uint32_t j1 = block_magic == 0u ? u : j;  // blocks of 16: 2^32 / 1 does not fit the multiplier
     if (t >= end) return -1;
-    const int at = selected[j1];
-    return at < 0 ? -1 : at * static_cast<int>(p.block) + t - static_cast<int>(j1) * static_cast<int>(p.block);
+    // t / block, exact below 2^28 (blocks of 16: 2^32 / 1 does not fit the multiplier)
+    const uint32_t u = static_cast<uint32_t>(t) >> 4;
+    const int j = static_cast<int>(plan.block_magic == 0u ? u : __umulhi(u, plan.block_magic));
+    const int at = selected[j], block = static_cast<int>(p.block);
+    return at < 0 ? -1 : at * block + t - j * block;
   }
 
   __device__ __forceinline__ uint32_t byte_of(int at) const {
@@ -682,11 +691,14 @@ struct Worker {
     return __all(fine);
   }
 
-  // rounds r0 .. r1 - 1 of the unit
+  // first position of the wave's step in round r, -1 if it has none
+  __device__ __forceinline__ int step_of(int r, int r1) const {
+    const int t = (r << plan.round_shift) + wave_k * T::kStep;
+    return r < r1 && t < end ? t : -1;
+  }
+
   __device__ __forceinline__ void walk(int r0, int r1) {
     if constexpr (kShared) {
-      __syncthreads();  // nobody reads the tiles of the unit before
-      stage((r0 * key_waves + wave_k) * T::kTileKeys, 0);
 #pragma unroll 1
       for (int r = r0; r < r1; ++r) {
         // this tile has arrived and the other one is read: no later request may still be under way here
@@ -706,16 +718,10 @@ struct Worker {
         }
       }
     } else {
-      auto first = [&](int r) {
-        const int t = r * plan.round_keys + wave_k * T::kStep;
-        return r < r1 && t < end ? t : -1;
-      };
-      int step = first(r0);
-      load_keys(step);
-      load_values(step);
+      int step = step_of(r0, r1);
 #pragma unroll 1
       for (int r = r0; step >= 0; ++r) {
-        const int next = first(r + 1);
+        const int next = step_of(r + 1, r1);
         if (kView == CacheView::kTree && step + T::kStep > len && !__all(values_finite())) advance<true>(step, next);
         else advance<false>(step, next);
         step = next;
@@ -859,7 +865,7 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
     const uint32_t n = uniform(rounds_of(p, plan, b));
     const uint32_t unit = (x - before) / n, r0 = x - before - unit * n;
     const uint32_t r1 = x1 - x < n - r0 ? r0 + (x1 - x) : n;
-    worker.begin(b, unit);
+    worker.begin(b, unit, r0, r1);
     worker.walk(r0, r1);
     // a part that begins the workgroup's stretch is its first, any other its last
     const int slot = blockIdx.x * 2 + (x == x0 ? 0 : 1);
@@ -895,7 +901,7 @@ struct Parts {
 __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
   constexpr int kAhead = 4;  // parts requested together
   const int lane = threadIdx.x & 63;
-  const int group = static_cast<int>(p.heads / p.heads_kv), rows = static_cast<int>(p.tokens) * group;
+  const int group = plan.group, rows = plan.rows;
   const int64_t at = blockIdx.x * static_cast<int64_t>(kThreads / 64) + uniform(threadIdx.x >> 6);
   const int64_t unit = at / plan.unit_rows, head = unit / plan.row_groups;
   if (head >= p.batch * p.heads_kv) return;
@@ -947,7 +953,7 @@ __device__ void add_weights(const CacheAttnParams& p, const CachePlan& plan, int
   __shared__ v2f stats_s[1024];
   const int64_t head = index / plan.weight_tiles;
   const int t0 = static_cast<int>(index - head * plan.weight_tiles) * kThreads * kWeightSteps + threadIdx.x;
-  const int group = static_cast<int>(p.heads / p.heads_kv);
+  const int group = plan.group;
   const int len = committed(p, head / p.heads_kv);
   if (t0 - static_cast<int>(threadIdx.x) >= len) return;
   const float* scratch = static_cast<const float*>(p.scratch);
@@ -1029,12 +1035,18 @@ CachePlan make_plan(const CacheAttnParams& p) {
   while (plan.row_waves < waves && plan.row_waves * 16 * plan.tiles < rows) plan.row_waves *= 2;
   plan.unit_rows = 16 * plan.tiles * plan.row_waves;
   plan.row_groups = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
-  plan.round_keys = (plan.shared ? 16384 / (dp * element) : element == 4 ? 16 : 32) * (waves / plan.row_waves);
+  const int round_keys =
+      (plan.shared ? 16384 / (dp * element) : element == 4 ? 16 : 32) * (waves / plan.row_waves);
+  plan.round_shift = __builtin_ctz(round_keys);
+  plan.group = static_cast<int>(p.heads / p.heads_kv);
+  plan.rows = static_cast<int>(rows);
+  plan.block_magic =
+      p.view == CacheView::kBlocks ? static_cast<uint32_t>(((1ull << 32) + p.block / 16 - 1) / (p.block / 16)) : 0u;
   plan.grid = plan.shared ? 256 : 512;
   plan.min_rounds = 1;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  plan.whole = walked <= plan.round_keys * 8 || units >= 2048;
+  plan.whole = (walked <= round_keys * 8 && p.view != CacheView::kDense) || units >= 2048;
   // scratch
   auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;

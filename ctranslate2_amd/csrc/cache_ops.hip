@@ -367,6 +367,14 @@ __global__ __launch_bounds__(kThreads) void block_bounds_kernel(CacheBoundsParam
   }
 }
 
+template <int kControl>
+__device__ __forceinline__ double dpp_double(double x) {
+  const int64_t bits = __double_as_longlong(x);
+  const int low = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), kControl, 0xf, 0xf, false);
+  const int high = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), kControl, 0xf, 0xf, false);
+  return __longlong_as_double(static_cast<int64_t>(high) << 32 | static_cast<uint32_t>(low));
+}
+
 // scores[b, hkv, j] = max over the group's heads of sum_d (q_d >= 0 ? q_d max_d : q_d min_d), NaN where
 // a bound is; float64, since a choice between blocks must not depend on how the sum was ordered. Eight
 // lanes per block, each with every eighth 16 bytes of its channels, kPair blocks at a time; the heads'
@@ -444,21 +452,38 @@ __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParam
               }
           }
       }
+      // The eight lanes add up and share out at once: half of the 16 sums go to the lane across (7 - i),
+      // half of the rest two lanes on, half of those to the neighbour; a lane ends with two heads of block
+      // u = its bits 2 and 1.
+      const bool upper = part & 4, second = part & 2, odd = part & 1;
+      double s8[2][kHeads], s4[kHeads], s2[2];
 #pragma unroll
-      for (int u = 0; u < kPair; ++u) {
-        const int j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
-          for (int o = 1; o < 8; o <<= 1) sum[u][h] += __shfl_xor(sum[u][h], o, 64);
-        int all = fine[u];
-        for (int o = 1; o < 8; o <<= 1) all &= __shfl_xor(all, o, 64);
-        if (part == 0 && j < to) {
-          double best = h0 ? p.scores[row * blocks + j] : sum[u][0];
+          s8[u][h] = (upper ? sum[2 + u][h] : sum[u][h]) + dpp_double<0x141>(upper ? sum[u][h] : sum[2 + u][h]);
 #pragma unroll
-          for (int h = 0; h < kHeads; ++h)
-            if (h < heads && (sum[u][h] > best || sum[u][h] != sum[u][h])) best = sum[u][h];
-          p.scores[row * blocks + j] = all ? best : __builtin_nan("");
-        }
+      for (int h = 0; h < kHeads; ++h)
+        s4[h] = (second ? s8[1][h] : s8[0][h]) + dpp_double<0x4e>(second ? s8[0][h] : s8[1][h]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        s2[h] = (odd ? s4[2 + h] : s4[h]) + dpp_double<0xb1>(odd ? s4[h] : s4[2 + h]);
+      int all = 0;
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) all |= fine[u] << u;
+      all &= __builtin_amdgcn_update_dpp(0, all, 0x141, 0xf, 0xf, false);
+      all &= __builtin_amdgcn_update_dpp(0, all, 0x4e, 0xf, 0xf, false);
+      all &= __builtin_amdgcn_update_dpp(0, all, 0xb1, 0xf, 0xf, false);
+      // the larger of two, NaN above all
+      auto larger = [](double a, double c) { return c > a || c != c ? c : a; };
+      double best = 2 * odd < heads ? s2[0] : -INFINITY;
+      if (2 * odd + 1 < heads) best = larger(best, s2[1]);
+      const double across = dpp_double<0xb1>(best);
+      best = odd ? best : larger(best, across);
+      const int u = part >> 1, j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
+      if (!odd && j < to) {
+        if (h0) best = larger(best, p.scores[row * blocks + j]);
+        p.scores[row * blocks + j] = all >> u & 1 ? best : __builtin_nan("");
       }
     }
   }
