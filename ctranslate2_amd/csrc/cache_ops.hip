@@ -95,11 +95,11 @@ struct Keys {
 // and the search ends with the byte whose bin is taken whole.
 template <typename K, typename F>
 __device__ int select_threshold(const Keys<K, F>& keys, int want, K* threshold) {
-  constexpr int kWaves = kSelectThreads / 64;
-  __shared__ uint32_t histogram[256];
+  constexpr int kWaves = kSelectThreads / 64, kBytes = sizeof(K);
+  __shared__ uint32_t histograms[kBytes][256];  // of every byte that a search may come to
   __shared__ K both_s[kWaves], none_s[kWaves];
-  __shared__ uint32_t digit_s, above_s, count_s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < kBytes * 256; i += kSelectThreads) histograms[i / 256][i % 256] = 0;
   K both = ~static_cast<K>(0), none = both;
   keys.each([&](int, K x, bool there) {
     both &= there ? x : ~static_cast<K>(0);
@@ -125,44 +125,36 @@ __device__ int select_threshold(const Keys<K, F>& keys, int want, K* threshold) 
   int upto = 64 - __clzll(static_cast<unsigned long long>(differ));  // bits below `upto` are searched
   K known = upto >= static_cast<int>(sizeof(K)) * 8 ? 0 : ~static_cast<K>(0) << upto;
   K prefix = both & known;
-  while (upto > 0) {
+  for (int pass = 0; upto > 0; ++pass) {
     const int bits = upto < 8 ? upto : 8, shift = upto - bits;
-    if (threadIdx.x < 256) histogram[threadIdx.x] = 0;
-    __syncthreads();
+    uint32_t* histogram = histograms[pass];
     keys.each([&](int, K x, bool there) {
       if (there && (x & known) == prefix)
         atomicAdd(&histogram[static_cast<uint32_t>(x >> shift) & ((1u << bits) - 1)], 1u);
     });
     __syncthreads();
-    if (wave == 0) {  // lane 0 has the four highest bins
-      uint32_t bin[4], sum = 0;
+    // every wave finds the bin by itself, lane 0 with the four highest
+    uint32_t bin[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += bin[i] = histogram[255 - 4 * lane - i];
-      const uint32_t upto_lane = wave_scan(sum);
-      const uint64_t reached = __ballot(upto_lane >= static_cast<uint32_t>(want));
-      if (lane == __builtin_ctzll(reached)) {
-        uint32_t above = upto_lane - sum, taken = bin[0];
-        int digit = 255 - 4 * lane;
+    for (int i = 0; i < 4; ++i) sum += bin[i] = histogram[255 - 4 * lane - i];
+    const uint32_t upto_lane = wave_scan(sum);
+    uint32_t above = upto_lane - sum, taken = bin[0];
+    int digit = 255 - 4 * lane;
 #pragma unroll
-        for (int i = 1; i < 4; ++i)
-          if (above + taken < static_cast<uint32_t>(want)) {
-            above += taken;
-            taken = bin[i];
-            digit = 255 - 4 * lane - i;
-          }
-        digit_s = digit;
-        above_s = above;
-        count_s = taken;
+    for (int i = 1; i < 4; ++i)
+      if (above + taken < static_cast<uint32_t>(want)) {
+        above += taken;
+        taken = bin[i];
+        digit = 255 - 4 * lane - i;
       }
-    }
-    __syncthreads();
-    want -= above_s;
-    prefix |= static_cast<K>(digit_s) << shift;
+    const int at = __builtin_ctzll(__ballot(upto_lane >= static_cast<uint32_t>(want)));
+    want -= __builtin_amdgcn_readlane(above, at);
+    prefix |= static_cast<K>(__builtin_amdgcn_readlane(digit, at)) << shift;
     known |= static_cast<K>((1u << bits) - 1) << shift;
     upto = shift;
     // Everything with this prefix is taken: nothing below it is, whatever its lower bits. (As a
     // threshold the prefix itself: it may be no key, then none is equal to it and all are above.)
-    if (count_s == static_cast<uint32_t>(want)) break;
+    if (__builtin_amdgcn_readlane(taken, at) == want) break;
   }
   *threshold = prefix;
   return want;
@@ -379,48 +371,60 @@ __device__ __forceinline__ double dpp_double(double x) {
 // a bound is; float64, since a choice between blocks must not depend on how the sum was ordered. Eight
 // lanes per block, each with every eighth 16 bytes of its channels, kPair blocks at a time; the heads'
 // queries wait in LDS as float64, split into max(q, 0) and min(q, 0): two products by converted bounds
-// instead of a choice per head. (An infinite bound times the zero half would be NaN: such blocks are
-// summed by the choice.) Bound by the float64 products and the LDS reads about as much as by the bounds.
+// instead of a choice per head. A bound that is not finite leaves no sum finite (0 x inf is NaN): such
+// blocks are summed again by the choice. Bound by the float64 products and the latency of two dependent
+// reads more than by the bounds' bytes.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParams p, int64_t blocks, int walkers) {
-  constexpr int V = 16 / sizeof(T), kHeads = 4, kPair = 4;  // heads, blocks at a time
+  constexpr int V = 16 / sizeof(T), kHeads = 4, kPair = 2, kBlocks = kThreads / 8;  // heads, blocks at a time
   __shared__ double2 q_s[kHeads][256];
   const int64_t row = blockIdx.x / walkers;
   const int64_t b = row / p.heads_kv, hkv = row % p.heads_kv;
   const int group = static_cast<int>(p.heads / p.heads_kv), dhead = static_cast<int>(p.dhead);
-  const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
-  const int count = static_cast<int>((n + p.block - 1) / p.block);
-  const int per = (count + walkers * kPair * 32 - 1) / (walkers * kPair * 32) * kPair * 32, from = static_cast<int>(blockIdx.x % walkers) * per;
-  const int to = from + per < count ? from + per : count;
-  if (from >= to || count <= p.top) return;  // (all blocks are taken: no scores are looked at)
+  const int n = static_cast<int>(clamped_length(p.lengths, p.length, b, p.t_max));
+  const int block = static_cast<int>(p.block), count = (n + block - 1) / block;
+  if (count <= p.top) return;  // (all blocks are taken: no scores are looked at)
   const int part = threadIdx.x & 7;
+  // the eight lanes' channels side by side: they are read together, from all banks
+  auto slot_of = [](int d) { return d / (8 * V) * (8 * V) + d % V * 8 + d / V % 8; };
   const T* bounds = static_cast<const T*>(p.bounds) + row * blocks * 2 * dhead;
   for (int h0 = 0; h0 < group; h0 += kHeads) {
     const int heads = group - h0 < kHeads ? group - h0 : kHeads;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kHeads * dhead; i += kThreads) {
-      const int h = i / dhead;
-      const double q = h < heads ? p.q[(b * p.heads + hkv * group + h0) * dhead + i] : 0.;
-      q_s[h][i - h * dhead] = q >= 0. ? double2{q, 0.} : q < 0. ? double2{0., q} : double2{q, q};
-    }
-    __syncthreads();
-    for (int j0 = from; j0 < to; j0 += kPair * kThreads / 8) {
+    for (int j0 = static_cast<int>(blockIdx.x % walkers) * kPair * kBlocks, first = j0; j0 < count;
+         j0 += walkers * kPair * kBlocks) {
       const T* low[kPair];
       double sum[kPair][kHeads] = {};
-      bool fine[kPair], finite = true;
 #pragma unroll
       for (int u = 0; u < kPair; ++u) {
-        const int j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
-        low[u] = bounds + static_cast<int64_t>(j < to ? j : to - 1) * 2 * dhead;
-        fine[u] = true;
+        const int j = j0 + u * kBlocks + (threadIdx.x >> 3);
+        low[u] = bounds + static_cast<int64_t>(j < count ? j : count - 1) * 2 * dhead;
+      }
+      int4 next[kPair][2];
+      auto request = [&](int d) {
+#pragma unroll
+        for (int u = 0; u < kPair; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            next[u][i] = *reinterpret_cast<const int4*>(low[u] + (d < dhead ? d : 0) + i * dhead);
+      };
+      request(part * V);
+      if (j0 == first) {  // (the first bounds are on their way while the queries are laid out)
+        if (h0) __syncthreads();
+        for (int i = threadIdx.x; i < kHeads * dhead; i += kThreads) {
+          const int h = i / dhead;
+          const double q = h < heads ? p.q[(b * p.heads + hkv * group + h0) * dhead + i] : 0.;
+          q_s[h][slot_of(i - h * dhead)] = q >= 0. ? double2{q, 0.} : q < 0. ? double2{0., q} : double2{q, q};
+        }
+        __syncthreads();
       }
       for (int d = part * V; d < dhead; d += 8 * V) {
         float x[kPair][V], y[kPair][V];
 #pragma unroll
         for (int u = 0; u < kPair; ++u) {
-          unpack<T>(*reinterpret_cast<const int4*>(low[u] + d), x[u]);
-          unpack<T>(*reinterpret_cast<const int4*>(low[u] + dhead + d), y[u]);
+          unpack<T>(next[u][0], x[u]);
+          unpack<T>(next[u][1], y[u]);
         }
+        request(d + 8 * V);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           double a[kPair], c[kPair];  // (converted once for all heads)
@@ -428,62 +432,61 @@ __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParam
           for (int u = 0; u < kPair; ++u) {
             a[u] = x[u][i];
             c[u] = y[u][i];
-            fine[u] &= !__builtin_isunordered(x[u][i], y[u][i]);
-            finite &= fabsf(x[u][i]) < INFINITY && fabsf(y[u][i]) < INFINITY;
           }
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
-            const double2 q = q_s[h][d + i];
+            const double2 q = q_s[h][slot_of(d + i)];
 #pragma unroll
             for (int u = 0; u < kPair; ++u) sum[u][h] = fma(q.y, a[u], fma(q.x, c[u], sum[u][h]));
           }
         }
       }
-      if (!__all(finite)) {
-#pragma unroll
-        for (int u = 0; u < kPair; ++u)
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) {
-            sum[u][h] = 0.;
-            for (int d = part * V; d < dhead; d += 8 * V)
-              for (int i = d; i < d + V; ++i) {
-                const double q = q_s[h][i].x + q_s[h][i].y;
-                sum[u][h] = fma(q, static_cast<double>(load_float(low[u][q >= 0. ? dhead + i : i])), sum[u][h]);
-              }
-          }
-      }
-      // The eight lanes add up and share out at once: half of the 16 sums go to the lane across (7 - i),
-      // half of the rest two lanes on, half of those to the neighbour; a lane ends with two heads of block
-      // u = its bits 2 and 1.
+      // The eight lanes add up and share out at once: a block's four sums to the lane across (7 - i) or
+      // kept, two of them two lanes on, one to the neighbour. A lane ends with head (bits 1, 0) of block
+      // (bit 2).
       const bool upper = part & 4, second = part & 2, odd = part & 1;
-      double s8[2][kHeads], s4[kHeads], s2[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
+      auto share = [&] {
+        double s4[kHeads], s2[2];
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
-          s8[u][h] = (upper ? sum[2 + u][h] : sum[u][h]) + dpp_double<0x141>(upper ? sum[u][h] : sum[2 + u][h]);
+          s4[h] = (upper ? sum[1][h] : sum[0][h]) + dpp_double<0x141>(upper ? sum[0][h] : sum[1][h]);
 #pragma unroll
-      for (int h = 0; h < kHeads; ++h)
-        s4[h] = (second ? s8[1][h] : s8[0][h]) + dpp_double<0x4e>(second ? s8[0][h] : s8[1][h]);
+        for (int h = 0; h < 2; ++h)
+          s2[h] = (second ? s4[2 + h] : s4[h]) + dpp_double<0x4e>(second ? s4[h] : s4[2 + h]);
+        return (odd ? s2[1] : s2[0]) + dpp_double<0xb1>(odd ? s2[0] : s2[1]);
+      };
+      double mine = share();
+      int nan = 0;  // bit u: block u has a NaN bound
+      if (!__all(fabs(mine) < INFINITY)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        s2[h] = (odd ? s4[2 + h] : s4[h]) + dpp_double<0xb1>(odd ? s4[h] : s4[2 + h]);
-      int all = 0;
+        for (int u = 0; u < kPair; ++u) {
 #pragma unroll
-      for (int u = 0; u < kPair; ++u) all |= fine[u] << u;
-      all &= __builtin_amdgcn_update_dpp(0, all, 0x141, 0xf, 0xf, false);
-      all &= __builtin_amdgcn_update_dpp(0, all, 0x4e, 0xf, 0xf, false);
-      all &= __builtin_amdgcn_update_dpp(0, all, 0xb1, 0xf, 0xf, false);
+          for (int h = 0; h < kHeads; ++h) sum[u][h] = 0.;
+          for (int d0 = part * V; d0 < dhead; d0 += 8 * V)
+            for (int d = d0; d < d0 + V; ++d) {
+              const float x = load_float(low[u][d]), y = load_float(low[u][dhead + d]);
+              nan |= __builtin_isunordered(x, y) ? 1 << u : 0;
+#pragma unroll
+              for (int h = 0; h < kHeads; ++h) {
+                const double2 q = q_s[h][slot_of(d)];
+                sum[u][h] = fma(q.x + q.y, static_cast<double>(q.y < 0. ? x : y), sum[u][h]);
+              }
+            }
+        }
+        mine = share();
+        nan |= __builtin_amdgcn_update_dpp(0, nan, 0x141, 0xf, 0xf, false);
+        nan |= __builtin_amdgcn_update_dpp(0, nan, 0x4e, 0xf, 0xf, false);
+        nan |= __builtin_amdgcn_update_dpp(0, nan, 0xb1, 0xf, 0xf, false);
+      }
       // the larger of two, NaN above all
       auto larger = [](double a, double c) { return c > a || c != c ? c : a; };
-      double best = 2 * odd < heads ? s2[0] : -INFINITY;
-      if (2 * odd + 1 < heads) best = larger(best, s2[1]);
-      const double across = dpp_double<0xb1>(best);
-      best = odd ? best : larger(best, across);
-      const int u = part >> 1, j = j0 + u * (kThreads / 8) + (threadIdx.x >> 3);
-      if (!odd && j < to) {
+      double best = (part & 3) < heads ? mine : -INFINITY;
+      best = larger(best, dpp_double<0xb1>(best));
+      best = larger(best, dpp_double<0x4e>(best));
+      const int j = j0 + (part >> 2) * kBlocks + (threadIdx.x >> 3);
+      if ((part & 3) == 0 && j < count) {
         if (h0) best = larger(best, p.scores[row * blocks + j]);
-        p.scores[row * blocks + j] = all >> u & 1 ? best : __builtin_nan("");
+        p.scores[row * blocks + j] = nan >> (part >> 2) & 1 ? __builtin_nan("") : best;
       }
     }
   }
@@ -525,7 +528,7 @@ void bounds_typed(const CacheBoundsParams& p, int64_t blocks, hipStream_t stream
 template <typename T>
 void scores_typed(const CacheSelectParams& p, int64_t blocks, hipStream_t stream) {
   const int64_t rows = p.batch * p.heads_kv;
-  const int walkers = walkers_for(rows, (blocks + kThreads / 2 - 1) / (kThreads / 2));
+  const int walkers = walkers_for(rows, (blocks + kThreads / 4 - 1) / (kThreads / 4));
   hipLaunchKernelGGL((block_scores_kernel<T>), dim3(static_cast<unsigned>(rows * walkers)), dim3(kThreads), 0, stream,
                      p, blocks, walkers);
 }
