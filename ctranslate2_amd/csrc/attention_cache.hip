@@ -460,29 +460,21 @@ struct Worker {
     return kAll & ~(old | seen);
   }
 
-  __device__ __forceinline__ static bool finite_word(uint32_t x) {
-    if constexpr (kType == kF32) return (x & 0x7f800000u) != 0x7f800000u;
+  // x with zeros in the place of what is not finite
+  __device__ __forceinline__ static uint32_t finite_part(uint32_t x) {
+    if constexpr (kType == kF32) return (x & 0x7f800000u) != 0x7f800000u ? x : 0u;
     constexpr uint32_t e = kType == kF16 ? 0x7c00u : 0x7f80u;
-    return (x & e) != e && (x >> 16 & e) != e;
+    return ((x & e) != e ? x & 0xffffu : 0u) | ((x >> 16 & e) != e ? x & 0xffff0000u : 0u);
   }
 
-  __device__ __forceinline__ bool values_finite() const {
-    bool fine = true;
-#pragma unroll
-    for (int j = 0; j < T::kLane; ++j)
-#pragma unroll
-      for (int h = 0; h < T::H; ++h)
-#pragma unroll
-        for (int w = 0; w < T::kWords; ++w) fine &= finite_word(v[j][h][w]);
-    return fine;
-  }
+  // first of the W neighbouring channels o[n][h W ..][i] that a lane has of a row
+  __device__ __forceinline__ int channel_of(int h, int i) const { return (h * 16 + i * 4 + g) * T::W; }
 
   // one step over positions step .. step + kStep - 1, whose keys and values are in registers or on
-  // their way; `next` is loaded as their registers come free (kShared: they are in `tile`). kApart: a
-  // drafted position among them holds values that are not finite.
-  template <bool kApart>
-  __device__ __forceinline__ void advance(int step, int next, const char* tile = nullptr, int first = 0) {
-    if constexpr (kShared) read_keys(tile, first);
+  // their way; `next` is loaded as their registers come free (kShared: they are in `tile`, the
+  // keys in registers; `more`: the tile holds another step)
+  __device__ __forceinline__ void advance(int step, int next, bool& not_finite, const char* tile = nullptr, int first = 0,
+                                          bool more = false) {
     float s[NT][T::kLane];
     {
       v4f acc[NT][T::kKeyTiles];
@@ -519,22 +511,37 @@ struct Worker {
 #pragma unroll
         for (int j = 0; j < T::kLane; ++j) s[n][j] = acc[n][j / 4][j % 4];
     }
-    if constexpr (!kShared) load_keys(next);
-    else if constexpr (!kApart) read_values(tile + T::kTileBytes, first);
+    if constexpr (kShared) {
+      read_values(tile + T::kTileBytes, first);
+      if (more) read_keys(tile, first + T::kStep);
+    } else {
+      load_keys(next);
+    }
 
-    uint32_t hidden[NT];  // bit j: the row does not see the lane's position j
-#pragma unroll
-    for (int n = 0; n < NT; ++n) hidden[n] = 0u;
     const int at = position(step + g * T::kLane);
     if (kView == CacheView::kBlocks ? !__all(at >= 0 && at + T::kLane <= len) : step + T::kStep > len) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         int row = row0 + n * 16 + c;
         rare(row);
-        hidden[n] = hidden_from(row, at);
+        const uint32_t hidden = hidden_from(row, at);
 #pragma unroll
         for (int j = 0; j < T::kLane; ++j)
-          if (hidden[n] >> j & 1) s[n][j] = -INFINITY;
+          if (hidden >> j & 1) s[n][j] = -INFINITY;
+      }
+      if constexpr (kView == CacheView::kTree) {
+        // a drafted position's NaN and infinite values would reach rows that do not see it as 0 x inf:
+        // they wait for add_not_finite()
+#pragma unroll
+        for (int j = 0; j < T::kLane; ++j)
+#pragma unroll
+          for (int h = 0; h < T::H; ++h)
+#pragma unroll
+            for (int w = 0; w < T::kWords; ++w) {
+              const uint32_t x = finite_part(v[j][h][w]);
+              not_finite |= x != v[j][h][w];
+              v[j][h][w] = x;
+            }
       }
     }
     if (kView == CacheView::kDense && p.weights) {
@@ -586,8 +593,7 @@ struct Worker {
       }
     }
 
-    if constexpr (kApart) add_values_apart(step, s, hidden);
-    else add_values(s);
+    add_values(s);
     if constexpr (!kShared) load_values(next);
   }
 
@@ -631,64 +637,46 @@ struct Worker {
     }
   }
 
-  // A drafted position holds NaN or infinite values that some rows must not see: 0 x inf would reach
-  // them through the matrix cores, so this step is added on the vector pipe, row by row.
-  __device__ void add_values_apart(int step, const float (&s)[NT][T::kLane], const uint32_t (&hidden)[NT]) {
+  // The NaN and infinite values of drafted positions, to the rows that see them. (A probability is above
+  // zero, so its product with them is what they are.)
+  __device__ void add_not_finite(int r0, int r1) {
+    constexpr int kStretch = kShared ? T::kTileKeys : T::kStep;  // of a wave in a round
 #pragma unroll 1
-    for (int key = 0; key < T::kStep; ++key) {
-      const int at = step + key, from = key / T::kLane * 16 + c, j = key % T::kLane;
-      if (at >= end) break;
-      const uint32_t row = byte_of(at);
-      float x[NT];
-      bool seen[NT];
+    for (int r = r0; r < r1; ++r) {
+      const int t = (r << plan.round_shift) + wave_k * kStretch, to = t + kStretch < end ? t + kStretch : end;
+#pragma unroll 1
+      for (int at = t < len ? len : t; at < to; ++at) {
+        bool seen[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        x[n] = s[n][0];
+        for (int n = 0; n < NT; ++n) seen[n] = !(hidden_from(row0 + n * 16 + c, at) & 1);
 #pragma unroll
-        for (int i = 1; i < T::kLane; ++i) x[n] = j == i ? s[n][i] : x[n];
-        x[n] = __shfl(x[n], from);
-        seen[n] = !(__shfl(hidden[n], from) >> j & 1);
-      }
+        for (int h = 0; h < T::H; ++h)
 #pragma unroll
-      for (int h = 0; h < T::H; ++h)
+          for (int i = 0; i < 4; ++i) {
+            // channels behind dhead read as zeros or as other channels: they are not stored
+            const uint32_t byte = byte_of(at) + channel_of(h, i) * T::kBytes;
+            v2u y[T::kWords / 2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // channels behind dhead read as zeros or as other channels: they are not stored
-          const uint32_t byte = row + (h * 16 + i * 4 + g) * T::W * T::kBytes;
-          v2u y[T::kWords / 2];
+            for (int w = 0; w < T::kWords / 2; ++w)
+              y[w] = __builtin_amdgcn_raw_buffer_load_b64(v_rsrc, byte + 8 * w, 0, 0);
 #pragma unroll
-          for (int w = 0; w < T::kWords / 2; ++w)
-            y[w] = __builtin_amdgcn_raw_buffer_load_b64(v_rsrc, byte + 8 * w, 0, 0);
+            for (int e = 0; e < T::W; ++e) {
+              float value;
+              if constexpr (kType == kF32) {
+                value = __uint_as_float(y[e >> 1][e & 1]);
+              } else {
+                const uint32_t bits = e & 1 ? y[e >> 2][e >> 1 & 1] >> 16 : y[e >> 2][e >> 1 & 1] & 0xffffu;
+                if constexpr (kType == kF16) value = __builtin_bit_cast(v2h, bits)[0];
+                else value = __uint_as_float(bits << 16);
+              }
+              const bool bad = !(fabsf(value) < INFINITY);
 #pragma unroll
-          for (int e = 0; e < T::W; ++e) {
-            float value;
-            if constexpr (kType == kF32) {
-              value = __uint_as_float(y[e >> 1][e & 1]);
-            } else {
-              const uint32_t bits = e & 1 ? y[e >> 2][e >> 1 & 1] >> 16 : y[e >> 2][e >> 1 & 1] & 0xffffu;
-              if constexpr (kType == kF16) value = __builtin_bit_cast(v2h, bits)[0];
-              else value = __uint_as_float(bits << 16);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float sum = fmaf(x[n], value, o[n][h * T::W + e][i]);
-              o[n][h * T::W + e][i] = seen[n] ? sum : o[n][h * T::W + e][i];
+              for (int n = 0; n < NT; ++n)
+                if (bad && seen[n]) o[n][h * T::W + e][i] += value;
             }
           }
-        }
+      }
     }
-  }
-
-  // whether a tile's values are all finite
-  __device__ __forceinline__ bool tile_finite(const char* tile) const {
-    bool fine = true;
-#pragma unroll 2
-    for (int i = lane * 16; i < T::kTileBytes; i += 1024) {
-      const v4u x = *reinterpret_cast<const v4u*>(tile + i);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) fine &= finite_word(x[w]);
-    }
-    return __all(fine);
   }
 
   // first position of the wave's step in round r, -1 if it has none
@@ -698,6 +686,7 @@ struct Worker {
   }
 
   __device__ __forceinline__ void walk(int r0, int r1) {
+    bool not_finite = false;
     if constexpr (kShared) {
 #pragma unroll 1
       for (int r = r0; r < r1; ++r) {
@@ -705,28 +694,23 @@ struct Worker {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         const int t = (r * key_waves + wave_k) * T::kTileKeys, buffer = (r - r0) & 1;
-        if (r + 1 < r1) stage(t + key_waves * T::kTileKeys, buffer ^ 1);
         const char* tile = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
-        if (t + T::kTileKeys > len && !tile_finite(tile + T::kTileBytes)) {
+        read_keys(tile, 0);
+        if (r + 1 < r1) stage(t + key_waves * T::kTileKeys, buffer ^ 1);
 #pragma unroll 1
-          for (int i = 0; i < T::kTileKeys; i += T::kStep)
-            if (t + i < end) advance<true>(t + i, 0, tile, i);
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < T::kTileKeys; i += T::kStep)
-            if (t + i < end) advance<false>(t + i, 0, tile, i);
-        }
+        for (int i = 0; i < T::kTileKeys && t + i < end; i += T::kStep)
+          advance(t + i, 0, not_finite, tile, i, i + T::kStep < T::kTileKeys);
       }
     } else {
       int step = step_of(r0, r1);
 #pragma unroll 1
       for (int r = r0; step >= 0; ++r) {
         const int next = step_of(r + 1, r1);
-        if (kView == CacheView::kTree && step + T::kStep > len && !__all(values_finite())) advance<true>(step, next);
-        else advance<false>(step, next);
+        advance(step, next, not_finite);
         step = next;
       }
     }
+    if (kView == CacheView::kTree && __any(not_finite)) add_not_finite(r0, r1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       l[n] = rows_sum(l[n]);
