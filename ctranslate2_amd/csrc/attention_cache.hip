@@ -17,9 +17,9 @@
 //                 channels of a position (256 bytes per 16 lanes) and MFMA number e takes the e-th of
 //                 each, so output row r of MFMA e is channel W r + e and nothing is transposed; the
 //                 16-bit types pair positions with one v_perm per register.
-// 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as two
-// 16-bit terms hi + lo, which leaves 2^-18 (bfloat16) / 2^-22 (float16) of them - the output is
-// float32, and one term would cost 2^-9. float32 caches use the float32 MFMA, nothing is rounded.
+// 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as a sum of
+// 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-11 (float16).
+// float32 caches use the float32 MFMA, nothing is rounded.
 //
 // Work is cut evenly whatever the lengths: the rounds (kStep positions per wave that shares a row
 // group) of all (entry, head, row group) units form one line, workgroup w of G takes the w-th G-th of
@@ -130,17 +130,21 @@ struct Mfma {  // 16-bit
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
                                                      0);
   }
-  // x = hi + lo up to half a step of lo, both pairs packed
-  static __device__ __forceinline__ void split(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  // the pair x0, x1 as a sum of kTerms pairs of 16-bit values, up to half a step of the last
+  template <int kTerms>
+  static __device__ __forceinline__ void split(float x0, float x1, uint32_t (&terms)[kTerms]) {
     v2f x = {x0, x1};
-    if constexpr (kType == kF16) {
-      const v2h h = __builtin_convertvector(x, v2h);
-      hi = __builtin_bit_cast(uint32_t, h);
-      lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(x - __builtin_convertvector(h, v2f), v2h));
-    } else {
-      const v2bf h = __builtin_convertvector(x, v2bf);
-      hi = __builtin_bit_cast(uint32_t, h);
-      lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(x - __builtin_convertvector(h, v2f), v2bf));
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t) {
+      if constexpr (kType == kF16) {
+        const v2h y = __builtin_convertvector(x, v2h);
+        terms[t] = __builtin_bit_cast(uint32_t, y);
+        x -= __builtin_convertvector(y, v2f);
+      } else {
+        const v2bf y = __builtin_convertvector(x, v2bf);
+        terms[t] = __builtin_bit_cast(uint32_t, y);
+        x -= __builtin_convertvector(y, v2f);
+      }
     }
   }
 };
@@ -211,7 +215,11 @@ struct Worker {
   __amdgpu_buffer_rsrc_t k_rsrc, v_rsrc;
   const int32_t* selected;
 
-  uint32_t q_hi[NT][T::kChunks][4], q_lo[NT][T::kHalf ? T::kChunks : 1][4];
+  // 16-bit terms of a query and of a probability. Three of bfloat16 carry float32; two leave 2^-18 of it,
+  // which is taken where the matrix cores bound the kernel (two row tiles of a wave: 1.5 times the products,
+  // and a third more registers than there are for the queries).
+  static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 && NT == 1 ? 3 : 2;
+  uint32_t queries[kTerms][NT][T::kChunks][4];
   float factor[NT];  // > 0: scores are factor times what the matrix cores give, to the base 2
   float m[NT], l[NT];  // m: without the factor until the walk ends
   v4f o[NT][T::E];
@@ -227,9 +235,6 @@ struct Worker {
     // row's four lanes hold neighbouring chunks and store whole lines together.
     chunk = (c & 3) * 4 + (c >> 2);
     const int wave = uniform(threadIdx.x >> 6);
-    // Two waves of a SIMD that run the same code in step want the matrix cores at the same time and
-    // leave them idle at the same time; the first one's priority keeps them apart.
-    if (kShared && wave < kWaves / 2) __builtin_amdgcn_s_setprio(1);
     wave_r = wave % plan.row_waves;
     wave_k = wave / plan.row_waves;
     key_waves = kWaves / plan.row_waves;
@@ -324,13 +329,17 @@ struct Worker {
 #pragma unroll
         for (int s = 0; s < T::kChunks; ++s)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, q_hi[n][s][j], q_lo[n][s][j]);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t terms[kTerms];
+            Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, terms);
+#pragma unroll
+            for (int t = 0; t < kTerms; ++t) queries[t][n][s][j] = terms[t];
+          }
       } else {
 #pragma unroll
         for (int s = 0; s < T::kChunks; ++s)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) q_hi[n][s][j] = __float_as_uint(x[s][j] * sign);
+          for (int j = 0; j < 4; ++j) queries[0][n][s][j] = __float_as_uint(x[s][j] * sign);
       }
       factor[n] = f < 1.17549435e-38f ? 1.17549435e-38f : f;  // (above zero: -inf times it stays -inf)
     }
@@ -475,6 +484,8 @@ struct Worker {
   // keys in registers; `more`: the tile holds another step)
   __device__ __forceinline__ void advance(int step, int next, bool& not_finite, const char* tile = nullptr, int first = 0,
                                           bool more = false) {
+    // (a wave in its products goes first, the SIMD's other one fills the gaps: 1 % of a long tree)
+    if constexpr (kShared) __builtin_amdgcn_s_setprio(1);
     float s[NT][T::kLane];
     {
       v4f acc[NT][T::kKeyTiles];
@@ -487,24 +498,20 @@ struct Worker {
       for (int x = 0; x < T::kChunks; ++x)
         if constexpr (T::kHalf) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int t = 0; t < kTerms; ++t)
 #pragma unroll
-            for (int i = 0; i < T::kKeyTiles; ++i)
-              acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{q_hi[n][x][0], q_hi[n][x][1], q_hi[n][x][2], q_hi[n][x][3]},
-                                           acc[n][i]);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < T::kKeyTiles; ++i)
-              acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{q_lo[n][x][0], q_lo[n][x][1], q_lo[n][x][2], q_lo[n][x][3]},
-                                           acc[n][i]);
+              for (int i = 0; i < T::kKeyTiles; ++i)
+                acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{queries[t][n][x][0], queries[t][n][x][1], queries[t][n][x][2], queries[t][n][x][3]},
+                                             acc[n][i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               acc[n][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[0][x][j]),
-                                                               __uint_as_float(q_hi[n][x][j]), acc[n][0], 0, 0, 0);
+                                                               __uint_as_float(queries[0][n][x][j]), acc[n][0], 0, 0, 0);
         }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -512,6 +519,7 @@ struct Worker {
         for (int j = 0; j < T::kLane; ++j) s[n][j] = acc[n][j / 4][j % 4];
     }
     if constexpr (kShared) {
+      __builtin_amdgcn_s_setprio(0);
       read_values(tile + T::kTileBytes, first);
       if (more) read_keys(tile, first + T::kStep);
     } else {
@@ -593,21 +601,23 @@ struct Worker {
       }
     }
 
+    if constexpr (kShared) __builtin_amdgcn_s_setprio(1);
     add_values(s);
+    if constexpr (kShared) __builtin_amdgcn_s_setprio(0);
     if constexpr (!kShared) load_values(next);
   }
 
   __device__ __forceinline__ void add_values(const float (&s)[NT][T::kLane]) {
     if constexpr (T::kHalf) {
-      v4u hi[NT], lo[NT];
+      v4u probability[kTerms][NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t a, d;
-          Mfma<kType>::split(s[n][2 * j], s[n][2 * j + 1], a, d);
-          hi[n][j] = a;
-          lo[n][j] = d;
+          uint32_t terms[kTerms];
+          Mfma<kType>::split(s[n][2 * j], s[n][2 * j + 1], terms);
+#pragma unroll
+          for (int t = 0; t < kTerms; ++t) probability[t][n][j] = terms[t];
         }
 #pragma unroll
       for (int h = 0; h < T::H; ++h)
@@ -619,9 +629,10 @@ struct Worker {
             a[w] = __builtin_amdgcn_perm(v[2 * w + 1][h][e >> 1], v[2 * w][h][e >> 1],
                                          e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) o[n][h * T::W + e] = Mfma<kType>::mul(a, hi[n], o[n][h * T::W + e]);
+          for (int t = 0; t < kTerms; ++t)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) o[n][h * T::W + e] = Mfma<kType>::mul(a, lo[n], o[n][h * T::W + e]);
+            for (int n = 0; n < NT; ++n)
+              o[n][h * T::W + e] = Mfma<kType>::mul(a, probability[t][n], o[n][h * T::W + e]);
         }
     } else {
 #pragma unroll
@@ -881,12 +892,15 @@ struct Parts {
   }
 };
 
-// One wave per row of a unit with several parts: out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i
+// out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i of the rows of units with several parts: 32 lanes per
+// row (64 for heads beyond 128 channels) with four channels each. One pass over the parts, four requested
+// together, their maximum kept as it grows: bound by the latency of two dependent reads (the record, the
+// parts), so that what counts is how many rows are on the chip at once.
 __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
-  constexpr int kAhead = 4;  // parts requested together
-  const int lane = threadIdx.x & 63;
-  const int group = plan.group, rows = plan.rows;
-  const int64_t at = blockIdx.x * static_cast<int64_t>(kThreads / 64) + uniform(threadIdx.x >> 6);
+  constexpr int kAhead = 4;
+  const int lanes = p.dhead > 128 ? 64 : 32, lane = threadIdx.x & (lanes - 1);
+  const int group = plan.group, rows = plan.rows, dhead = static_cast<int>(p.dhead);
+  const int64_t at = blockIdx.x * static_cast<int64_t>(kThreads / lanes) + threadIdx.x / lanes;
   const int64_t unit = at / plan.unit_rows, head = unit / plan.row_groups;
   if (head >= p.batch * p.heads_kv) return;
   const int local = static_cast<int>(at - unit * plan.unit_rows);
@@ -896,23 +910,25 @@ __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
   if (parts.count == 1) return;
   const float* scratch = static_cast<const float*>(p.scratch);
   const v2f* ml = reinterpret_cast<const v2f*>(scratch + plan.parts_ml);
-  float most = -INFINITY;
-  for (int i = lane; i < parts.count; i += 64) most = fmaxf(most, ml[parts.row(plan, i, local)][0]);
-  most = wave_max(most);
-  const float base = finite_base(most);
-  float total = 0.f;
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int channel = lane * 4 < dhead ? lane * 4 : 0;
+  float most = -INFINITY, total = 0.f;
+  v4f o = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < parts.count; i0 += kAhead) {
     v2f part[kAhead];
-    float x[kAhead][4];
+    v4f x[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int64_t from = parts.row(plan, i0 + u < parts.count ? i0 + u : 0, local);
+      const int64_t from = parts.row(plan, i0 + u < parts.count ? i0 + u : i0, local);
       part[u] = ml[from];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        x[u][c] = c * 64 + lane < p.dhead ? scratch[plan.parts_o + from * p.dhead + c * 64 + lane] : 0.f;
+      x[u] = *reinterpret_cast<const v4f*>(scratch + plan.parts_o + from * dhead + channel);
     }
+    float higher = most;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) higher = fmaxf(higher, part[u][0]);
+    const float base = finite_base(higher), keep = shift_of(most, base);
+    total *= keep;
+    o *= keep;
+    most = higher;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (i0 + u >= parts.count) break;
@@ -925,10 +941,8 @@ __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
   const float by = total == 0.f ? 0.f : 1.f / total;
   const int64_t b = head / p.heads_kv, hkv = head - b * p.heads_kv;
   const int i = row / group;
-  float* to = p.out + ((b * p.tokens + i) * p.heads + hkv * group + row - i * group) * p.dhead;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (c * 64 + lane < p.dhead) to[c * 64 + lane] = total == 0.f ? 0.f : o[c] * by;
+  float* to = p.out + ((b * p.tokens + i) * p.heads + hkv * group + row - i * group) * dhead;
+  if (lane * 4 < dhead) *reinterpret_cast<v4f*>(to + lane * 4) = total == 0.f ? v4f{0.f, 0.f, 0.f, 0.f} : o * by;
 }
 
 // weights[b, hkv, t] += sum over the group's heads of exp(s_t - m) / l
@@ -1046,7 +1060,8 @@ CachePlan make_plan(const CacheAttnParams& p) {
     plan.scores = plan.stats + up(p.batch * p.heads * 2);
     plan.total = plan.scores + p.batch * p.heads * plan.score_pitch;
   }
-  plan.join_groups = plan.whole ? 0 : static_cast<int>((units * plan.unit_rows + kThreads / 64 - 1) / (kThreads / 64));
+  const int join_rows = kThreads / (p.dhead > 128 ? 64 : 32);
+  plan.join_groups = plan.whole ? 0 : static_cast<int>((units * plan.unit_rows + join_rows - 1) / join_rows);
   plan.weight_tiles =
       p.weights ? static_cast<int>((p.t_max + kThreads * kWeightSteps - 1) / (kThreads * kWeightSteps)) : 0;
   return plan;

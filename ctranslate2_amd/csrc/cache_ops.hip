@@ -37,10 +37,22 @@ __device__ __forceinline__ int64_t clamped_length(const int32_t* lengths, int64_
   return n < 0 ? 0 : (n > t_max ? t_max : n);
 }
 
-template <typename K>
-__device__ __forceinline__ K wave_and(K x) {
-  for (int o = 32; o > 0; o >>= 1) x &= static_cast<K>(__shfl_xor(static_cast<unsigned long long>(x), o, 64));
-  return x;
+__device__ __forceinline__ uint32_t wave_and(uint32_t x) {
+  auto meet = [&](auto ctrl, auto rows) {
+    x &= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(-1, static_cast<int>(x), decltype(ctrl)::value,
+                                                           decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  meet(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());
+  meet(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  meet(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  meet(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  meet(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());
+  meet(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ uint64_t wave_and(uint64_t x) {
+  return static_cast<uint64_t>(wave_and(static_cast<uint32_t>(x >> 32))) << 32 | wave_and(static_cast<uint32_t>(x));
 }
 
 // Keys 0 .. n - 1 spread over a workgroup: every wave has a stretch of them, its lanes the positions
