@@ -7,7 +7,7 @@
 // l = 0 and an output of zero. Positions that a row does not see never enter a sum, whatever they
 // hold.
 //
-// Matrix cores, no LDS on the way. A wave takes kStep positions and NT tiles of 16 rows:
+// Matrix cores. A wave takes kStep positions and NT tiles of 16 rows:
 //   S^T = K Q^T   the key rows as they lie in memory are the A operand, rows of q the columns of B;
 //                 a lane then holds kLane consecutive positions of one row (its column), so that
 //                 the row's maximum and rescaling are the lane's own but for two lane swaps;
@@ -17,6 +17,17 @@
 //                 channels of a position (256 bytes per 16 lanes) and MFMA number e takes the e-th of
 //                 each, so output row r of MFMA e is channel W r + e and nothing is transposed; the
 //                 16-bit types pair positions with one v_perm per register.
+// Up to 32 rows (a decode step, a small tree) every wave loads its own positions straight into the
+// operands' registers, the next step's requested as they come free: bound by the reads. From 33 rows on,
+// heads of up to 128 channels: tiles of 16 KB of keys and of values in LDS, filled by loads that bypass the
+// registers, one tile ahead, shared by four or eight waves of 16 or 32 rows each: bound by the matrix cores
+// (and, on short caches, by a workgroup's way in and out: queries split, parts written and joined).
+// Measured, with finish_kernel: 32 entries of 5.2 k positions on average, 8 heads of 128 bfloat16, one
+// token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 199 us, 0.98 PFLOP/s of
+// 16-bit products (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26 tokens: 61 us. Four tiles per
+// wave without LDS took 452 us on the second (outputs and queries need all 512 registers and spill),
+// values by the transposing LDS read instead of v_perm 220 against 207.
+//
 // 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as a sum of
 // 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-11 (float16).
 // float32 caches use the float32 MFMA, nothing is rounded.
@@ -220,6 +231,9 @@ struct Worker {
   // and a third more registers than there are for the queries).
   static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 && NT == 1 ? 3 : 2;
   uint32_t queries[kTerms][NT][T::kChunks][4];
+  // Probabilities are 2^(s + kLift - reference): the reference is a maximum that later ones exceed by up to
+  // kSlack, so that outputs are rescaled seldom, and float16, whose steps end at 2^-24, takes them 2^6 larger.
+  static constexpr float kSlack = 8.f, kLift = kType == kF16 ? 6.f : 0.f;
   float factor[NT];  // > 0: scores are factor times what the matrix cores give, to the base 2
   float m[NT], l[NT];  // m: without the factor until the walk ends
   v4f o[NT][T::E];
@@ -568,9 +582,7 @@ struct Worker {
       }
     }
 
-    // A maximum that grew by less than kSlack (to the base 2) stays the reference: probabilities up to
-    // 2^kSlack fit every type, and outputs are rescaled seldom.
-    constexpr float kSlack = 8.f;
+    // a maximum that grew by less than kSlack stays the reference
     float most[NT];
     bool grown = false;
 #pragma unroll
@@ -593,7 +605,7 @@ struct Worker {
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float base = finite_base(m[n]) * factor[n];
+      const float base = finite_base(m[n]) * factor[n] - kLift;
 #pragma unroll
       for (int j = 0; j < T::kLane; ++j) {
         s[n][j] = __builtin_amdgcn_exp2f(fmaf(s[n][j], factor[n], -base));
@@ -702,8 +714,7 @@ struct Worker {
 #pragma unroll 1
       for (int r = r0; r < r1; ++r) {
         // this tile has arrived and the other one is read: no later request may still be under way here
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\ns_barrier" ::: "memory");
         const int t = (r * key_waves + wave_k) * T::kTileKeys, buffer = (r - r0) & 1;
         const char* tile = lds + (wave_k * 2 + buffer) * 2 * T::kTileBytes;
         read_keys(tile, 0);
@@ -725,7 +736,7 @@ struct Worker {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       l[n] = rows_sum(l[n]);
-      if (m[n] != -INFINITY) m[n] *= factor[n];
+      if (m[n] != -INFINITY) m[n] = m[n] * factor[n] - kLift;
     }
   }
 

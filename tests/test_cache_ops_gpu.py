@@ -150,6 +150,9 @@ TREES = [
     (1, 3, 71, 1, 64, [90], 4),
     (1, 64, 8, 2, 128, [1500], 11),
     (1, 2, 2, 1, 96, [4097], 5),
+    (1, 600, 4, 1, 64, [100], 3),
+    (150, 2, 2, 1, 32, [1 + 13 * (i % 7) * (i % 11) for i in range(150)], 2),  # more entries than lanes
+    (300, 1, 8, 8, 16, [i % 5 for i in range(300)], 1),  # more units than the line takes
 ]
 
 
@@ -236,6 +239,19 @@ def test_tree_queries_of_any_size(gpu, dtype, size):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", (3, 40))
+@pytest.mark.parametrize("scale", (0.0, -0.3))
+def test_tree_scales(gpu, dtype, tokens, scale):
+    """Scale zero weighs all that is seen alike, a negative one turns the order round."""
+    gen, rng = generator(8), np.random.default_rng(8)
+    k, v = make_cache(gen, dtype, 1, 1, 400, 64)
+    q = torch.randn((1, tokens, 2, 64), device="cuda", generator=gen)
+    seen = tree_mask(rng, 1, tokens)
+    got = run_tree(q, k, v, dtype, None, 333, to_words(seen), scale)
+    check_tree(got, q, k, v, dtype, [333], seen, scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_tree_peaked_rows(gpu, dtype):
     """One key far above the others (a sink), early or late; the rest must not be lost or doubled."""
     gen = generator(6)
@@ -287,6 +303,7 @@ def run_accumulate(q, k, v, dtype, lengths, length, scale, weights, stream=None,
 ACCUMULATE = [
     (1, 1, 1, 8, [0]), (2, 8, 8, 64, [1, 333]), (3, 8, 2, 128, [0, 65, 1000]), (2, 20, 4, 80, [77, 500]),
     (1, 71, 1, 64, [130]), (1, 16, 16, 256, [300]), (1, 4, 2, 128, [9000]), (5, 4, 1, 96, [31, 32, 33, 64, 1]),
+    (130, 2, 1, 16, [i % 9 * 40 for i in range(130)]), (260, 8, 8, 8, [i % 4 * 7 for i in range(260)]),
 ]
 
 
@@ -494,6 +511,8 @@ BLOCKS = [
     (2, 4, 1, 96, 3000, 16, 40, 2, 3, [2999, 17]),
     (1, 8, 2, 128, 20000, 16, 300, 1, 2, [19999]),
     (1, 2, 2, 200, 300, 32, 64, 4, 4, [300]),
+    (1, 2, 1, 8, 300000, 16, 5, 1, 1, [299990]),  # more blocks than the selection keeps in registers
+    (90, 4, 1, 16, 400, 16, 6, 1, 1, [i % 10 * 40 for i in range(90)]),
 ]
 
 
@@ -543,6 +562,26 @@ def test_blocks_ties_and_nan_bounds(gpu, dtype):
         see[:, j * block:(j + 1) * block] = True
     want, tol, _ = reference(q[0], k[0, 0], v[0, 0], see, 0.125, dtype)
     within(got[0], want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_blocks_infinite_bounds(gpu, dtype):
+    """Infinite keys bound by infinity: taken first where a query leans to them, last where it leans away."""
+    gen = generator(44)
+    block, dhead = 16, 64
+    n = block * 30
+    k, v = make_cache(gen, dtype, 1, 1, n, dhead)
+    k[0, 0, 16 * 7 + 3, 5] = float("inf")
+    k[0, 0, 16 * 11:16 * 12, 6] = float("-inf")
+    q = torch.randn((1, 3, dhead), device="cuda", generator=gen)
+    q[0, :, 5] = 1.0
+    q[0, :, 6] = 1.0
+    q[0, 2, 5] = -1.0
+    bounds = torch.empty((1, 1, 30, 2, dhead), dtype=k.dtype, device="cuda")
+    run_bounds(k, dtype, None, None, n, block, bounds)
+    _, selected = run_blocks(q, k, v, dtype, bounds, None, n, block, 12, 0, 0, 0.125)
+    keep = select_reference(q[0], bounds[0, 0], n, block, 12, 0, 0)
+    assert selected[0, 0].tolist() == keep and 7 in keep and 11 not in keep
 
 
 @pytest.mark.parametrize("dtype", TYPES)
