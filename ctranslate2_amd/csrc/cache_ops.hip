@@ -70,10 +70,17 @@ struct Keys {
     lane = threadIdx.x & 63;
     from = wave * stretch;
     to = from + stretch < n ? from + stretch : n;
+    // all at once for a long stretch (requests without a branch between them), what there is of a short one
+    const bool few = stretch <= 4 * 64;
 #pragma unroll
-    for (int u = 0; u < kKeep; ++u) {
-      const int i = from + u * 64 + lane;
-      kept[u] = key(i < to ? i : 0);
+    for (int u = 0; u < kKeep; ++u) kept[u] = 0;
+    if (few) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (from + u * 64 < to) kept[u] = key(from + u * 64 + lane < to ? from + u * 64 + lane : 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kKeep; ++u) kept[u] = key(from + u * 64 + lane < to ? from + u * 64 + lane : 0);
     }
   }
   // visit(i, key(i), whether there is an i), whole waves at a time
