@@ -904,11 +904,11 @@ struct Parts {
 };
 
 // out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i of the rows of units with several parts: 32 lanes per
-// row (64 for heads beyond 128 channels) with four channels each. One pass over the parts, four requested
+// row (64 for heads beyond 128 channels) with four channels each. One pass over the parts, eight requested
 // together, their maximum kept as it grows: bound by the latency of two dependent reads (the record, the
 // parts), so that what counts is how many rows are on the chip at once.
 __device__ void join_rows(const CacheAttnParams& p, const CachePlan& plan) {
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 8;
   const int lanes = p.dhead > 128 ? 64 : 32, lane = threadIdx.x & (lanes - 1);
   const int group = plan.group, rows = plan.rows, dhead = static_cast<int>(p.dhead);
   const int64_t at = blockIdx.x * static_cast<int64_t>(kThreads / lanes) + threadIdx.x / lanes;
@@ -1039,7 +1039,7 @@ CachePlan make_plan(const CacheAttnParams& p) {
   // eight waves with rows of their own share (16 each up to 64 rows, 32 beyond).
   plan.shared = p.view == CacheView::kTree && rows > 32 && dp <= 128;
   const int waves = waves_of(plan.shared);
-  plan.tiles = plan.shared && rows > 64 ? 2 : 1;
+  plan.tiles = plan.shared && rows > 128 ? 2 : 1;
   plan.row_waves = plan.shared ? 4 : 1;
   while (plan.row_waves < waves && plan.row_waves * 16 * plan.tiles < rows) plan.row_waves *= 2;
   plan.unit_rows = 16 * plan.tiles * plan.row_waves;
@@ -1052,7 +1052,8 @@ CachePlan make_plan(const CacheAttnParams& p) {
   plan.block_magic =
       p.view == CacheView::kBlocks ? static_cast<uint32_t>(((1ull << 32) + p.block / 16 - 1) / (p.block / 16)) : 0u;
   plan.grid = plan.shared ? 256 : 512;
-  plan.min_rounds = 1;
+  // 128 positions at least where a part is many rows
+  plan.min_rounds = plan.shared ? std::max(1, 128 / round_keys) : 1;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
   plan.whole = (walked <= round_keys * 8 && p.view != CacheView::kDense) || units >= 2048;
