@@ -20,11 +20,12 @@
 // Up to 32 rows (a decode step, a small tree) every wave loads its own positions straight into the
 // operands' registers, the next step's requested as they come free: bound by the reads. From 33 rows on,
 // heads of up to 128 channels: tiles of 16 KB of keys and of values in LDS, filled by loads that bypass the
-// registers, one tile ahead, shared by four or eight waves of 16 or 32 rows each: bound by the matrix cores
-// (and, on short caches, by a workgroup's way in and out: queries split, parts written and joined).
+// registers, one tile ahead, shared by four or eight waves of 16 rows each up to 128 rows, of 32 beyond: bound
+// by the matrix cores (and, on short caches, by a workgroup's way in and out: queries split, parts written and
+// joined).
 // Measured, with finish_kernel: 32 entries of 5.2 k positions on average, 8 heads of 128 bfloat16, one
 // token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 199 us, 0.98 PFLOP/s of
-// 16-bit products (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26 tokens: 61 us. Four tiles per
+// 16-bit products (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26 tokens: 54 us. Four tiles per
 // wave without LDS took 452 us on the second (outputs and queries need all 512 registers and spill),
 // values by the transposing LDS read instead of v_perm 220 against 207.
 //
@@ -1036,7 +1037,9 @@ CachePlan make_plan(const CacheAttnParams& p) {
   const int64_t rows = p.tokens * (p.heads / p.heads_kv);
   const int dp = padded_head(p.dhead), element = p.kv_dtype == kF32 ? 4 : 2;
   // Few rows: every wave loads for itself. From 33 on, heads of up to 128: tiles in LDS, which four or
-  // eight waves with rows of their own share (16 each up to 64 rows, 32 beyond).
+  // eight waves with rows of their own share, 16 each up to 128 rows, 32 beyond. bfloat16, heads of 128, 16
+  // entries of 1.1 k on average, four rows a token: 8 tokens 33.4 us apart, 38.3 shared, 16 tokens 48.8 and
+  // 40.3; 33 tokens 87.9 us by 16 rows, 69.0 by 32, 26 tokens 54 and 61.
   plan.shared = p.view == CacheView::kTree && rows > 32 && dp <= 128;
   const int waves = waves_of(plan.shared);
   plan.tiles = plan.shared && rows > 128 ? 2 : 1;
@@ -1056,7 +1059,16 @@ CachePlan make_plan(const CacheAttnParams& p) {
   plan.min_rounds = plan.shared ? std::max(1, 128 / round_keys) : 1;
   const int64_t walked = p.view == CacheView::kBlocks ? p.top * p.block : p.t_max;
   const int64_t units = p.batch * p.heads_kv * plan.row_groups;
-  plan.whole = (walked <= round_keys * 8 && p.view != CacheView::kDense) || units >= 2048;
+  // A workgroup alone with its unit writes no parts, and a tree's call is then one launch; the line keeps the
+  // workgroups even where units are few or long. Rounds up to which the former was the faster, for less than
+  // 192 units, less than 512 and more; heads of 128, us, line / alone, units and positions (bfloat16):
+  // tree 4 tokens, 64 x 512: 14.1 / 13.4, 192 x 1020: 30.0 / 22.0, 512 x 2044: 70.8 / 63.4; 24 tokens,
+  // 64 x 1020: 31 / 48, 512 x 1532: 146 / 120; blocks 64 x 1024: 29 / 41, 512 x 1024: 76 / 74;
+  // accumulate 192 x 250: 15.2 / 13.3, 512 x 1000: 39 / 36.
+  static constexpr int kAlone[3][3] = {{2, 8, 16}, {2, 4, 32}, {8, 16, 32}};
+  const int many = units >= 512 ? 2 : units >= 192 ? 1 : 0;
+  const int view = p.view == CacheView::kDense ? 0 : p.view == CacheView::kBlocks ? 1 : 2;
+  plan.whole = walked <= round_keys * kAlone[view][many] || units >= 2048;
   // scratch
   auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;
