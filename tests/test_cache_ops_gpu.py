@@ -763,3 +763,47 @@ def test_repeated_calls_give_the_same_bits(gpu):
     first = run_tree(q, k, v, "bf16", lengths, 0, None, 0.09).clone()
     for _ in range(5):
         assert torch.equal(first, run_tree(q, k, v, "bf16", lengths, 0, None, 0.09))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch", (24, 65))
+def test_many_units_of_several_rounds(gpu, dtype, batch):
+    """Enough (entry, head) units that a workgroup takes one from end to end, over several rounds and
+    lengths that end inside them; every view, a sample of the entries."""
+    gen, rng = generator(91), np.random.default_rng(91)
+    heads, heads_kv, dhead, t_max, scale = 16, 8, 64, 640, 0.125
+    lengths = [int(rng.integers(0, 600)) for _ in range(batch)]
+    lengths[:3] = [600, 0, 1]
+    sample = (0, 1, 2, batch // 2, batch - 1)
+    given = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for tokens in (3, 20):
+        k, v = make_cache(gen, dtype, batch, heads_kv, t_max, dhead, [n + tokens for n in lengths])
+        q = torch.randn((batch, tokens, heads, dhead), device="cuda", generator=gen) * 2
+        seen = tree_mask(rng, batch, tokens)
+        got = run_tree(q, k, v, dtype, given, 0, to_words(seen), scale)
+        check_tree(got, q, k, v, dtype, lengths, seen, scale, sample)
+    k, v = make_cache(gen, dtype, batch, heads_kv, 270, dhead, [min(n, 270) for n in lengths])
+    q = torch.randn((batch, heads, dhead), device="cuda", generator=gen) * 2
+    weights = torch.zeros((batch, heads_kv, 270), device="cuda")
+    got = run_accumulate(q, k, v, dtype, given, 0, scale, weights)
+    block, top = 16, 12
+    bounds = torch.full((batch, heads_kv, -(-270 // block), 2, dhead), float("nan"), dtype=k.dtype, device="cuda")
+    run_bounds(k, dtype, None, given, 0, block, bounds)
+    some, selected = run_blocks(q, k, v, dtype, bounds, given, 0, block, top, 1, 2, scale)
+    for b in sample:
+        n = min(lengths[b], 270)
+        for g in range(heads_kv):
+            rows = q[b, 2 * g:2 * g + 2]
+            see = torch.ones((2, n), dtype=torch.bool, device="cuda")
+            want, tol, p = reference(rows, k[b, g, :n], v[b, g, :n], see, scale, dtype)
+            within(got[b, 2 * g:2 * g + 2], want, tol, "entry %d group %d" % (b, g))
+            if n:
+                within(weights[b, g, :n], p[0][0] + p[1][0], p[0][1] + p[1][1] + (p[0][0] + p[1][0]) * 3 * 2.0 ** -24,
+                       "weights of entry %d group %d" % (b, g))
+            keep = select_reference(rows, bounds[b, g], n, block, top, 1, 2)
+            assert selected[b, g].tolist() == keep + [-1] * (top - len(keep))
+            see[:] = False
+            for j in keep:
+                see[:, j * block:(j + 1) * block] = True
+            want, tol, _ = reference(rows, k[b, g, :n], v[b, g, :n], see, scale, dtype)
+            within(some[b, 2 * g:2 * g + 2], want, tol, "blocks of entry %d group %d" % (b, g))
