@@ -227,10 +227,10 @@ struct Worker {
   __amdgpu_buffer_rsrc_t k_rsrc, v_rsrc;
   const int32_t* selected;
 
-  // 16-bit terms of a query and of a probability. Three of bfloat16 carry float32; two leave 2^-18 of it,
-  // which is taken where the matrix cores bound the kernel (two row tiles of a wave: 1.5 times the products,
-  // and a third more registers than there are for the queries).
-  static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 && NT == 1 ? 3 : 2;
+  // 16-bit terms of a query and of a probability: three of bfloat16 and two of float16 carry float32. Two of
+  // bfloat16 (2^-18) and 32 rows a wave took 200 us where 16 rows and three take 305 (4 entries of 23 k, 64
+  // tokens), with an error twice that of float32 arithmetic (4.6e-6): not taken.
+  static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 ? 3 : 2;
   uint32_t queries[kTerms][NT][T::kChunks][4];
   // Probabilities are 2^(s + kLift - reference): the reference is a maximum that later ones exceed by up to
   // kSlack, so that outputs are rescaled seldom, and float16, whose steps end at 2^-24, takes them 2^6 larger.
@@ -1037,12 +1037,17 @@ CachePlan make_plan(const CacheAttnParams& p) {
   const int64_t rows = p.tokens * (p.heads / p.heads_kv);
   const int dp = padded_head(p.dhead), element = p.kv_dtype == kF32 ? 4 : 2;
   // Few rows: every wave loads for itself. From 33 on, heads of up to 128: tiles in LDS, which four or
-  // eight waves with rows of their own share, 16 each up to 128 rows, 32 beyond. bfloat16, heads of 128, 16
-  // entries of 1.1 k on average, four rows a token: 8 tokens 33.4 us apart, 38.3 shared, 16 tokens 48.8 and
-  // 40.3; 33 tokens 87.9 us by 16 rows, 69.0 by 32, 26 tokens 54 and 61.
+  // eight waves with rows of their own share. bfloat16, heads of 128, 16 entries of 1.1 k on average, four rows a
+  // token: 8 tokens 33.4 us apart, 38.3 shared; 16 tokens 48.8 and 40.3.
   plan.shared = p.view == CacheView::kTree && rows > 32 && dp <= 128;
   const int waves = waves_of(plan.shared);
-  plan.tiles = plan.shared && rows > 128 ? 2 : 1;
+  // 32 rows a wave read the tiles half as often, 16 have a shorter way in and out: the former where there are
+  // rows for eight such waves and enough positions times rows. float16, heads of 128, 64 tokens, us by 16 / 32:
+  // 4 entries of 500 30.7 / 42.9, 4 of 2000 48 / 59, 4 of 8000 107 / 103, 16 of 8000 356 / 306; float32 51 / 70,
+  // 104 / 119, 314 / 313, 1139 / 1060. Three bfloat16 terms of 32 rows of 128 channels are more than the
+  // registers: 16 of 8000 take 414 us by 16, 518 by 32.
+  const bool long_tree = rows > 128 && rows * p.t_max * p.heads_kv * p.batch >= 60000000;
+  plan.tiles = plan.shared && long_tree && (p.kv_dtype != kBF16 || dp <= 64) ? 2 : 1;
   plan.row_waves = plan.shared ? 4 : 1;
   while (plan.row_waves < waves && plan.row_waves * 16 * plan.tiles < rows) plan.row_waves *= 2;
   plan.unit_rows = 16 * plan.tiles * plan.row_waves;
@@ -1119,7 +1124,8 @@ void launch_head(const CacheAttnParams& p, const CachePlan& plan, hipStream_t st
   if (p.view == CacheView::kDense) return launch_tiles<kType, DP, 1, CacheView::kDense>(p, plan, stream);
   if (p.view == CacheView::kBlocks) return launch_tiles<kType, DP, 1, CacheView::kBlocks>(p, plan, stream);
   if constexpr (DP < 256) {
-    if (plan.shared && plan.tiles == 2) return launch_tiles<kType, DP, 2, CacheView::kTree, true>(p, plan, stream);
+    if constexpr (kType != kBF16 || DP <= 64)
+      if (plan.tiles == 2) return launch_tiles<kType, DP, 2, CacheView::kTree, true>(p, plan, stream);
     if (plan.shared) return launch_tiles<kType, DP, 1, CacheView::kTree, true>(p, plan, stream);
   }
   launch_tiles<kType, DP, 1, CacheView::kTree>(p, plan, stream);
@@ -1136,12 +1142,14 @@ void launch_typed(const CacheAttnParams& p, const CachePlan& plan, hipStream_t s
 }  // namespace
 
 int64_t cache_attention_scratch_bytes(const CacheAttnParams& p) {
-  // the types differ in their rounds: as much as the larger takes
+  // the types differ in their rounds and tiles: as much as the largest takes
+  int64_t most = 0;
   CacheAttnParams other = p;
-  other.kv_dtype = kF32;
-  const int64_t a = make_plan(other).total;
-  other.kv_dtype = kBF16;
-  return std::max(a, make_plan(other).total) * 4;
+  for (int type : {kF32, kF16, kBF16}) {
+    other.kv_dtype = type;
+    most = std::max(most, make_plan(other).total);
+  }
+  return most * 4;
 }
 
 void launch_cache_attention(const CacheAttnParams& p, hipStream_t stream) {

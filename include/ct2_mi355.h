@@ -542,10 +542,8 @@ int ct2x_attention_full_half(const float* d_q, const float* d_k, const float* d_
  * otherwise). What lies behind an entry's positions is never looked at: it may hold anything.
  * Scores, softmax statistics and sums are fp32. Products with 16-bit caches run on the 16-bit matrix
  * cores, the fp32 operand (query, probability) as a sum of 16-bit terms: two of float16 (2^-22 of it
- * left), three of bfloat16 (2^-27); more than 128 rows (tokens * heads / heads_kv) of bfloat16 and
- * heads of up to 128 channels in a tree take two (2^-18). What a row sees is to be finite: an infinite
- * or NaN query, key or value leaves infinities or NaN in the rows that see it. A row that sees nothing
- * gets an output of zero.
+ * left), three of bfloat16 (2^-27). What a row sees is to be finite: an infinite or NaN query, key or
+ * value leaves infinities or NaN in the rows that see it. A row that sees nothing gets an output of zero.
  * d_scratch: at least the *_scratch_bytes() of the same sizes (-1: the sizes are refused, see
  * ct2x_last_error), content irrelevant before and after; one call at a time may use it, calls on one
  * stream may share it. Calls enqueue kernels only and may be captured into a graph. */
