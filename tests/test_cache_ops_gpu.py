@@ -5,8 +5,8 @@ Tolerance of an attention output, per element. A score s = scale sum_d q_d k_d i
 product and sum of fp32 rounds by at most 2^-24 relative, and the roundings are independent, so six
 standard deviations of d of them are within 6 sqrt(d) 2^-24 of scale |q o k|_2 (in quadrature: each
 partial sum is at most of the size of the terms' 2-norm up to sqrt(d)); a query enters the matrix cores
-of a 16-bit type as two terms, each rounded to half a step, which leaves 2^-18 (bfloat16) or 2^-22
-(float16) of it; the exponent's argument s log2(e) rounds at 2^-24 |s|, twice. A probability then is off by 2 ds
+of a 16-bit type as three terms (bfloat16) or two (float16), each rounded to half a step, which leaves
+2^-27 or 2^-22 of it; the exponent's argument s log2(e) rounds at 2^-24 |s|, twice. A probability then is off by 2 ds
 relative (its own exponential and the sum's), plus the same split of the probability, plus an
 exponential and n additions in fp32. So |out - exact| <= (2 ds + split + 2^-20 + 6 sqrt(n) 2^-24) sum_t p_t |v_t|.
 Choices, moves and bounds are exact."""
@@ -21,7 +21,7 @@ from ctranslate2_amd import _lib
 pytestmark = pytest.mark.gpu
 
 TYPES = {"f32": (0, torch.float32), "f16": (4, torch.float16), "bf16": (5, torch.bfloat16)}
-SPLIT = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -18}
+SPLIT = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -27}
 GUARD = 64  # elements behind every output that no call may touch
 
 
@@ -807,3 +807,25 @@ def test_many_units_of_several_rounds(gpu, dtype, batch):
                 see[:, j * block:(j + 1) * block] = True
             want, tol, _ = reference(rows, k[b, g, :n], v[b, g, :n], see, scale, dtype)
             within(some[b, 2 * g:2 * g + 2], want, tol, "blocks of entry %d group %d" % (b, g))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dhead, tokens, heads, lengths, t_max", [
+    (64, 40, 16, [900, 33, 0], 31500), (128, 33, 8, [65, 4000], 114000), (80, 130, 4, [511], 116000),
+], ids=str)
+def test_tree_in_a_large_cache(gpu, dtype, dhead, tokens, heads, lengths, t_max):
+    """Many rows in a cache with room for many positions: 32 rows a wave. Any mask, rows that see nothing,
+    drafted tokens that no row sees hold anything."""
+    gen, rng = generator(93), np.random.default_rng(93)
+    batch, heads_kv = len(lengths), 2
+    k, v = make_cache(gen, dtype, batch, heads_kv, t_max, dhead, [n + tokens for n in lengths])
+    q = torch.randn((batch, tokens, heads, dhead), device="cuda", generator=gen) * 2
+    seen = tree_mask(rng, batch, tokens)
+    seen[0, 3] = rng.random(tokens) < 0.3
+    seen[-1, 1] = seen[-1, 32] = False
+    seen[:, :, 5] = False
+    for b, n in enumerate(lengths):
+        k[b, :, n + 5], v[b, :, n + 5] = float("nan"), float("inf")
+    given = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = run_tree(q, k, v, dtype, given, 0, to_words(seen), dhead ** -0.5)
+    check_tree(got, q, k, v, dtype, lengths, seen, dhead ** -0.5)
