@@ -20,14 +20,15 @@
 // Up to 32 rows (a decode step, a small tree) every wave loads its own positions straight into the
 // operands' registers, the next step's requested as they come free: bound by the reads. From 33 rows on,
 // heads of up to 128 channels: tiles of 16 KB of keys and of values in LDS, filled by loads that bypass the
-// registers, one tile ahead, shared by four or eight waves of 16 rows each up to 128 rows, of 32 beyond: bound
-// by the matrix cores (and, on short caches, by a workgroup's way in and out: queries split, parts written and
-// joined).
+// registers, one tile ahead, shared by four or eight waves of 16 rows each, of 32 in long calls (make_plan):
+// bound by the matrix cores (and, on short caches, by a workgroup's way in and out: queries split, parts
+// written and joined).
 // Measured, with finish_kernel: 32 entries of 5.2 k positions on average, 8 heads of 128 bfloat16, one
-// token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 199 us, 0.98 PFLOP/s of
-// 16-bit products (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26 tokens: 54 us. Four tiles per
-// wave without LDS took 452 us on the second (outputs and queries need all 512 registers and spill),
-// values by the transposing LDS read instead of v_perm 220 against 207.
+// token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 297 us, 0.98 PFLOP/s of
+// 16-bit products, six for each of the formula's (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26
+// tokens: 54 us. Tried with two terms of bfloat16 on the second, where they and 32 rows a wave took 200 us:
+// four row tiles per wave without LDS 452 us (outputs and queries need all 512 registers and spill), values by
+// the transposing LDS read instead of v_perm 220 against 207.
 //
 // 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as a sum of
 // 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-11 (float16).

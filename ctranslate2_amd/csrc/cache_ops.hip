@@ -220,7 +220,8 @@ __device__ int emit_selected(const Keys<K, F>& keys, K threshold, int ties, G em
   return all + (all_equal < ties ? all_equal : ties);
 }
 
-// positions[b, hkv, :]: what stays, ascending, -1 behind the last
+// positions[b, hkv, :]: what stays, ascending, -1 behind the last. One workgroup per row: bound by the
+// latency of its passes (64 rows of 16 k weights: 16 us; histograms split by lane took the same).
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvictParams p) {
   const int64_t row = blockIdx.x, b = row / p.heads_kv;
   const int n = static_cast<int>(clamped_length(p.lengths, p.length, b, p.t_max));
@@ -243,7 +244,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvict
 // A workgroup moves one cache line (128 bytes) of the kept rows of a (entry, head)'s keys or values,
 // kMoveSteps rows per thread between two barriers. Rows only ever move to the front, so that the rows
 // of a step are read before any later step's place is written: one workgroup that takes all steps in
-// turn may write where it reads. Apart, `chunks` workgroups take the steps.
+// turn may write where it reads. Apart, `chunks` workgroups take the steps. Bound by the copy: 64 rows of
+// 4096 kept positions of 128 bfloat16 apart 56 us, 4.8 TB/s.
 constexpr int kMoveThreads = 512, kMoveSteps = 4;
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(CacheEvictParams p, int row_bytes, int slices,
                                                                   int chunks) {
@@ -318,7 +320,8 @@ __device__ __forceinline__ void unpack(const int4& x, float (&y)[16 / sizeof(T)]
 
 // A wave per (entry, head, block): 16 bytes of a row per lane, lanes of the same channels joined by
 // lane exchanges. Rows behind the end repeat the last one, which changes no minimum. minimum /
-// maximum hand on a NaN, and every bound is a key's value, so the way back to 16 bits is exact.
+// maximum hand on a NaN, and every bound is a key's value, so the way back to 16 bits is exact. Bound by
+// the reads: 4 entries of up to 32 k positions, 8 heads of 128 float16: 39.6 us, 5.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void block_bounds_kernel(CacheBoundsParams p, int64_t blocks, int walkers,
                                                                 int lanes) {
@@ -392,7 +395,9 @@ __device__ __forceinline__ double dpp_double(double x) {
 // queries wait in LDS as float64, split into max(q, 0) and min(q, 0): two products by converted bounds
 // instead of a choice per head. A bound that is not finite leaves no sum finite (0 x inf is NaN): such
 // blocks are summed again by the choice. Bound by the float64 products and the latency of two dependent
-// reads more than by the bounds' bytes.
+// reads more than by the bounds' bytes: 8 entries of 1024 blocks, 32 / 8 heads of 128 bfloat16 11 us, the
+// choice after it 7.4. (Both in one workgroup per row, for few blocks: no faster, 22.4 us for the whole call
+// at 129 blocks either way, and 3 % slower from 128 channels on.)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParams p, int64_t blocks, int walkers) {
   constexpr int V = 16 / sizeof(T), kHeads = 4, kPair = 2, kBlocks = kThreads / 8;  // heads, blocks at a time
