@@ -137,6 +137,25 @@ def _declare_cache_ops(L):
     for name, sizes in (("tree", 6), ("accumulate", 5), ("blocks", 7)):
         f = getattr(L, "ct2x_attention_%s_scratch_bytes" % name)
         f.restype, f.argtypes = N, [N] * sizes
+    L.ct2x_cache_evict = _without_workspace(L.ct2x_cache_evict)
+
+
+def _without_workspace(call):
+    """`call` with the tail of the family's attention calls, (.., d_scratch, scratch_bytes, stream),
+    accepted beside its own (.., stream): an eviction needs no workspace, a serving loop that hands its own
+    to every call of a step may do so here too. Any other number of arguments is an error; ctypes passes
+    surplus ones on, and the first would be taken for the stream."""
+    own = len(call.argtypes)
+
+    def with_either_tail(*args):
+        if len(args) == own + 2:
+            args = args[:-3] + args[-1:]
+        elif len(args) != own:
+            raise TypeError("%s takes %d arguments, or %d with a workspace (%d given)" %
+                            (call.__name__, own, own + 2, len(args)))
+        return call(*args)
+
+    return with_either_tail
 
 
 def check(rc):
