@@ -185,16 +185,16 @@ def prepare(case, seed):
     if case["op"] == "blocks":
         s["bounds"] = _all_bounds(s["k"], s["lengths"], case["block"])
         s["selected"] = torch.empty((b, hkv, case["top"]), dtype=torch.int32, device="cuda")
-    if case["op"] in ("tree", "accumulate", "blocks"):
+    if case["op"] in ("tree", "accumulate", "evict", "blocks"):
         # the workspace of a serving loop: as large as any call of these sizes asks for
         s["scratch"] = torch.empty(_scratch_bytes(case), dtype=torch.uint8, device="cuda")
     return s
 
 
 def _scratch_bytes(case):
-    rows = case["batch"] * case.get("tokens", 1) * case["heads"]
+    rows = case["batch"] * case.get("tokens", 1) * case.get("heads", case["heads_kv"])
     partials = (rows * 64 + 131072) * (case["dhead"] + 4) * 4
-    scores = case["batch"] * case["heads"] * (_t_max(case) + 64) * 8
+    scores = case["batch"] * case.get("heads", case["heads_kv"]) * (_t_max(case) + 64) * 8
     return partials + scores + (1 << 20)
 
 
@@ -370,7 +370,7 @@ def _own_evict(s):
     _lib.check(_lib.lib().ct2x_cache_evict(
         p(s["k"]), p(s["v"]), _TYPE_IDS[c["dtype"]], p(s["weights"]), p(s["lengths"]), 0, c["batch"], c["heads_kv"],
         c["dhead"], s["t_max"], c["budget"], c["recent"], c["budget"], p(s["k_out"]), p(s["v_out"]),
-        p(s["weights_out"]), p(s["positions"]), p(s["lengths_out"]), None))
+        p(s["weights_out"]), p(s["positions"]), p(s["lengths_out"]), p(s["scratch"]), s["scratch"].numel(), None))
     return [s["k_out"], s["v_out"], s["weights_out"], s["positions"], s["lengths_out"]]
 
 
