@@ -555,17 +555,19 @@ struct Worker {
       }
       if constexpr (kView == CacheView::kTree) {
         // a drafted position's NaN and infinite values would reach rows that do not see it as 0 x inf:
-        // they wait for add_not_finite()
+        // they wait for add_not_finite(); those of the committed ones before it every row sees
 #pragma unroll
-        for (int j = 0; j < T::kLane; ++j)
+        for (int j = 0; j < T::kLane; ++j) {
+          const bool drafted = at + j >= len;
 #pragma unroll
           for (int h = 0; h < T::H; ++h)
 #pragma unroll
             for (int w = 0; w < T::kWords; ++w) {
-              const uint32_t x = finite_part(v[j][h][w]);
+              const uint32_t x = drafted ? finite_part(v[j][h][w]) : v[j][h][w];
               not_finite |= x != v[j][h][w];
               v[j][h][w] = x;
             }
+        }
       }
     }
     if (kView == CacheView::kDense && p.weights) {
