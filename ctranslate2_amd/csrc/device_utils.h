@@ -225,8 +225,8 @@ __device__ __forceinline__ float expf_glibc(float x) { return exact_expf_glibc(x
 // one final rounding. The reference's CPU LogSoftMax ends with std::log(exp_sum)
 // (src/cpu/kernels.cc:449); glibc's logf is NOT correctly rounded (0.17 percent of inputs differ
 // from the rounded double log), and a one-ulp shift of a whole log-probability row is enough to
-// swap near-tied beams. The constants were read out of the libm.so.6 of the authoring image
-// (glibc 2.35) and the restatement checked bit for bit against it on 5e5 inputs. x must be a
+// swap near-tied beams. The constants are that published source's table (logf_data.c); the result
+// is logf's of glibc 2.35 bit for bit on 5e5 inputs. x must be a
 // positive normal float (a softmax denominator is >= 1).
 __device__ __forceinline__ float logf_glibc(float x) {
   static constexpr double kTab[16][2] = {
