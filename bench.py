@@ -348,10 +348,11 @@ def ragged_leg(translator, args):
 
 def tp_local_leg(model_dir, sources, kw, ref_hyps):
     """Tensor parallelism on the ONE visible GPU: the model sharded over 2 ranks that live as threads
-    of this process (in-process communicator), row-parallel layers exchanged through the one-shot
-    mailbox kernels (tp_oneshot.hip) - the code path a multi-GPU node runs over xGMI, minus the
-    links. Reports tokens/s of the sharded decode (NOT a scaling number: both ranks share one GPU),
-    whether its tokens equal the unsharded engine's, and the loopback price of one exchange pair."""
+    of this process (in-process communicator), row-parallel layers exchanged by its collectives, which
+    meet on the host. Reports tokens/s of the sharded decode (NOT a scaling number: both ranks share one
+    GPU), whether its tokens equal the unsharded engine's, and the loopback price of one exchange pair
+    through the one-shot mailbox kernels (tp_oneshot.hip), the code path of a multi-GPU node minus the
+    links - tp_shm_leg decodes through those, between two processes."""
     import ctypes as C
     import threading
     import ctranslate2_amd as ct2
@@ -384,11 +385,11 @@ def tp_local_leg(model_dir, sources, kw, ref_hyps):
     L = _lib.lib()
     _lib.check(L.ct2x_tp_selftest_oneshot(0, 2, C.c_int64(32), C.c_int64(256), C.c_int64(512), 200, C.byref(us)))
     return {"workload": "same model and batch, tensor parallel x2 as two in-process ranks on this one GPU "
-                        "(one-shot mailbox exchanges; functional leg, not a scaling number)",
+                        "(collectives that meet on the host; functional leg, not a scaling number)",
             "value": tokens / max(dt0, dt1), "unit": "tokens/s",
             "tokens_equal_unsharded": bool(hyps0 == ref_hyps and hyps1 == ref_hyps),
             "exchange_pair_us_loopback": us.value,
-            "collective_calls_per_row_parallel_dense": 0, "device_side_exchanges_per_row_parallel_dense": 2}
+            "collective_calls_per_row_parallel_dense": 2, "device_side_exchanges_per_row_parallel_dense": 0}
 
 
 def tp_shm_leg(model_dir, args, ref_hyps):

@@ -639,14 +639,18 @@ int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t 
   API_TRY
   // The one-shot exchanges of a row-parallel int8 Dense (tp_oneshot.hip) on the in-process
   // communicator: `world` rank threads, each with a [rows, depth] slice of one activation and its
-  // own int32 partial product [rows, n]. Checked against what ONE device computes from the whole
+  // own int32 partial product [rows, n]. Their kernels wait for each other, so the two streams are a pair
+  // that was seen to run at the same time, and the ranks meet on the host before the first exchange:
+  // everything is set up by then, and no call that could sit in a queue behind a waiting kernel is made
+  // before both ranks' exchanges are enqueued. Checked against what ONE device computes from the whole
   // row (global absmax -> scale -> Quantize; sum of the partials -> Dequantize): every rank must
   // hold identical, bit-exact results. Then `iters` exchange pairs are timed per rank (HIP events
   // on the rank's stream; all ranks run concurrently) - the single-device loopback price of the
   // two exchanges, reported as the maximum over the ranks.
-  CT2X_CHECK(world == 2, "ct2x_tp_selftest_oneshot: the in-process form has two ranks (see make_local_comms)");
+  CT2X_CHECK(world == 2, "ct2x_tp_selftest_oneshot: the in-process form has two ranks");
   CT2X_CHECK(tp_oneshot_fits(rows, rows * n), "ct2x_tp_selftest_oneshot: message larger than the mailbox");
-  auto comms = make_local_comms(world);
+  CT2X_HIP_CHECK(hipSetDevice(device_index));
+  auto comms = make_local_comms(world, /*mailboxes=*/true);
   CT2X_CHECK(comms[0]->peer_box() != nullptr, "one-shot mailboxes are disabled (CT2X_TP_ONESHOT=0)");
   std::vector<std::string> errors(world);
   std::vector<float> us(world, 0.f);
@@ -659,6 +663,17 @@ int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t 
     h_ws[j] = 50.f + static_cast<float>(j % 97);
     h_bias[j] = static_cast<float>(j % 13) * 0.01f;
   }
+  hipStream_t streams[2];
+  make_concurrent_streams(streams);
+  std::atomic<int> arrived{0};
+  std::atomic<bool> failed{false};
+  auto meet = [&](int times) {  // the ranks' host threads, for the times-th time
+    arrived.fetch_add(1);
+    while (arrived.load() < times * world) {
+      if (failed.load()) throw Error("the other rank failed");
+      std::this_thread::yield();
+    }
+  };
   std::vector<std::thread> threads;
   std::vector<std::vector<float>> outs(world);
   std::vector<std::vector<int8_t>> qouts(world);
@@ -666,7 +681,11 @@ int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t 
     threads.emplace_back([&, r] {
       try {
         CT2X_HIP_CHECK(hipSetDevice(device_index));
-        hipStream_t stream = thread_stream_with_priority(r);
+        hipStream_t stream = streams[r];
+        set_active_stream(stream);
+        hipEvent_t e0, e1;
+        CT2X_HIP_CHECK(hipEventCreate(&e0));
+        CT2X_HIP_CHECK(hipEventCreate(&e1));
         const TpPeerBox& pb = *comms[r]->peer_box();
         std::vector<float> xs(static_cast<size_t>(rows) * depth);
         for (int64_t i = 0; i < rows; ++i)
@@ -686,30 +705,32 @@ int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t 
         CT2X_HIP_CHECK(hipMemcpyAsync(dp, part.data(), part.size() * 4, hipMemcpyHostToDevice, stream));
         CT2X_HIP_CHECK(hipMemcpyAsync(dws, h_ws.data(), n * 4, hipMemcpyHostToDevice, stream));
         CT2X_HIP_CHECK(hipMemcpyAsync(dbias, h_bias.data(), n * 4, hipMemcpyHostToDevice, stream));
-        launch_tp_amax_quantize(pb, dx, rows, depth, 3, dq, ds, stream);
-        launch_tp_sum_dequant(pb, dp, ds, dws, dbias, nullptr, rows, n, dy, stream);
         outs[r].resize(part.size());
         qouts[r].resize(xs.size());
+        CT2X_HIP_CHECK(hipStreamSynchronize(stream));
+        meet(1);
+        launch_tp_amax_quantize(pb, dx, rows, depth, 3, dq, ds, stream);
+        launch_tp_sum_dequant(pb, dp, ds, dws, dbias, nullptr, rows, n, dy, stream);
+        meet(2);
         CT2X_HIP_CHECK(hipMemcpyAsync(outs[r].data(), dy, part.size() * 4, hipMemcpyDeviceToHost, stream));
         CT2X_HIP_CHECK(hipMemcpyAsync(qouts[r].data(), dq, xs.size(), hipMemcpyDeviceToHost, stream));
         CT2X_HIP_CHECK(hipStreamSynchronize(stream));
+        meet(3);
         if (iters > 0) {
-          hipEvent_t e0, e1;
-          CT2X_HIP_CHECK(hipEventCreate(&e0));
-          CT2X_HIP_CHECK(hipEventCreate(&e1));
           CT2X_HIP_CHECK(hipEventRecord(e0, stream));
           for (int it = 0; it < iters; ++it) {
             launch_tp_amax_quantize(pb, dx, rows, depth, 3, dq, ds, stream);
             launch_tp_sum_dequant(pb, dp, ds, dws, dbias, nullptr, rows, n, dy, stream);
           }
           CT2X_HIP_CHECK(hipEventRecord(e1, stream));
+          meet(4);
           CT2X_HIP_CHECK(hipStreamSynchronize(stream));
           float ms = 0.f;
           CT2X_HIP_CHECK(hipEventElapsedTime(&ms, e0, e1));
           us[r] = ms * 1e3f / static_cast<float>(iters);
-          (void)hipEventDestroy(e0);
-          (void)hipEventDestroy(e1);
         }
+        (void)hipEventDestroy(e0);
+        (void)hipEventDestroy(e1);
         TpBoxControl ctl;
         CT2X_HIP_CHECK(hipMemcpy(&ctl, pb.box[r], sizeof(ctl), hipMemcpyDeviceToHost));
         if (ctl.status != 0) throw Error("a poll of the one-shot exchange gave up (peer never arrived)");
@@ -719,10 +740,13 @@ int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t 
           device_free(ptr);
       } catch (const std::exception& e) {
         errors[r] = e.what();
+        failed.store(true);
       }
+      set_active_stream(nullptr);
     });
   }
   for (auto& th : threads) th.join();
+  for (hipStream_t s : streams) (void)hipStreamDestroy(s);
   for (int r = 0; r < world; ++r)
     CT2X_CHECK(errors[r].empty(), "rank " + std::to_string(r) + ": " + errors[r]);
   // reference: what one device computes from the whole rows (same formulas, host arithmetic)

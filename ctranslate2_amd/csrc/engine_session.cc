@@ -87,8 +87,6 @@ std::unique_ptr<DecodeState> Engine::start(const int32_t* src_ids, const int32_t
   auto st = std::make_unique<DecodeState>();
   st->engine = this;
   st->stream = thread_stream();  // the calling (worker) thread's stream: sessions run concurrently
-  if (tp_ && tp_->peer_box() && std::string(tp_->backend()) == "in-process")
-    st->stream = thread_stream_with_priority(tp_->rank());  // (ranks on one GPU: distinct queues)
   tls_stream = st->stream;
   set_active_stream(tls_stream);
   st->batch = batch;

@@ -610,7 +610,7 @@ void Engine::step(DecodeState& st, bool graph) {
   // Under tensor parallelism the step is captured when the communicator's collectives are plain
   // stream work (RCCL); the in-process test double rendezvous on the host and runs eagerly.
   // (with mailboxes, a step whose exchanges all fit the one-shot form contains no collective call at
-  // all - that also makes the in-process communicator capturable)
+  // all - that also makes the shared-memory communicator capturable)
   bool tp_stream_only = tp_ && tp_->capturable();
   if (tp_ && !tp_stream_only && tp_->peer_box() && !tp_fast_) {
     int64_t widest = dec_.d_model;

@@ -229,7 +229,7 @@ public:
     CT2X_HIP_CHECK(hipEventCreateWithFlags(&s_->ready[rank], hipEventDisableTiming));
     CT2X_HIP_CHECK(hipEventCreateWithFlags(&s_->done[rank], hipEventDisableTiming));
   }
-  // (the boxes are allocated by make_local_comms once every rank exists)
+  // (the boxes, if any, are allocated by make_local_comms once every rank exists)
   void set_boxes() {
     pb_.rank = rank_;
     pb_.world = s_->world;
@@ -561,19 +561,16 @@ std::shared_ptr<TpComm> make_rccl_comm(int rank, int world, const void* unique_i
   return std::make_shared<RcclComm>(rank, world, unique_id);
 }
 
-std::vector<std::shared_ptr<TpComm>> make_local_comms(int world) {
+std::vector<std::shared_ptr<TpComm>> make_local_comms(int world, bool mailboxes) {
   if (world < 1 || world > 8) throw Error("in-process communicator: world size must be 1..8");
   auto shared = std::make_shared<LocalShared>(world);
   std::vector<std::shared_ptr<TpComm>> comms;
   std::vector<std::shared_ptr<LocalComm>> locals;
   for (int r = 0; r < world; ++r) locals.push_back(std::make_shared<LocalComm>(shared, r));
   const char* e = std::getenv("CT2X_TP_ONESHOT");
-  if (world == 2 && !(e && e[0] == '0')) {
-    // the same mailboxes and kernels as between GPUs, on one device: what the single-GPU box can
-    // verify of the one-shot exchanges (protocol, tags, parity, exactness) and time as a loopback.
-    // TWO ranks only: their kernels wait for each other, so they must sit on different hardware
-    // queues - guaranteed by giving the two rank threads streams of different priority
-    // (thread_stream_with_priority); more in-process ranks keep the host-rendezvous collectives.
+  if (mailboxes && !(e && e[0] == '0')) {
+    // the same mailboxes and kernels as between GPUs, on one device: what a single GPU can verify of
+    // the one-shot exchanges (protocol, tags, parity, exactness) and time as a loopback
     for (int r = 0; r < world; ++r) {
       CT2X_HIP_CHECK(hipMalloc(reinterpret_cast<void**>(&shared->boxes[r]), tp_box_bytes()));
       CT2X_HIP_CHECK(hipMemset(shared->boxes[r], 0, tp_box_bytes()));

@@ -25,8 +25,8 @@ namespace ct2x {
 
 // ---- one-shot exchanges over peer-mapped mailboxes (tp_oneshot.hip) ---------------------------
 // Every rank owns one mailbox ("box") that every other rank can store into: peer-mapped device
-// memory between GPUs (hipIpc handles exchanged at bootstrap), plain device memory for the
-// in-process communicator. Layout: control block | absmax granules [2 parity][R sources][rows] |
+// memory between GPUs or processes (hipIpc handles exchanged at bootstrap); plain device memory for the
+// self test that runs two ranks in one process. Layout: control block | absmax granules [2 parity][R sources][rows] |
 // sum granules [2 parity][R sources][elements]; a granule is 8 bytes {payload, tag}.
 constexpr int kTpMaxWorld = 8;
 constexpr int64_t kTpBoxMaxRows = 4096;            // rows per absmax exchange
@@ -92,6 +92,14 @@ std::shared_ptr<TpComm> make_rccl_comm(int rank, int world, const void* unique_i
 std::shared_ptr<TpComm> make_shm_comm(int rank, int world, const std::string& name);
 
 // `world` communicators sharing one rendezvous object; comm i must be used by exactly one thread.
-std::vector<std::shared_ptr<TpComm>> make_local_comms(int world);
+// Their collectives meet on the host: no kernel waits for another rank's, whatever hardware queues the
+// ranks' streams share (a process has few). `mailboxes`: with boxes on the current device for the one-shot
+// kernels - for a caller that keeps every other call away while those wait for each other
+// (ct2x_tp_selftest_oneshot); an engine does not, its sessions allocate and copy between launches.
+std::vector<std::shared_ptr<TpComm>> make_local_comms(int world, bool mailboxes = false);
+
+// Two streams of the current device whose kernels run at the same time: tried out by two kernels that
+// meet within a few milliseconds or give up, on new streams until a pair does. The caller destroys them.
+void make_concurrent_streams(hipStream_t (&streams)[2]);
 
 }  // namespace ct2x

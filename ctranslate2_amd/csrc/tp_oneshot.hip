@@ -7,8 +7,8 @@
 //   (1) before its GEMM: the max over ranks of every row's absmax (the global Quantize scale);
 //   (2) after its GEMM:  the sum over ranks of the exact int32 partial products.
 // Both travel as 8-byte GRANULES {payload, tag} written by ONE system-scope store each into the
-// receiver's mailbox (xGMI peer store between GPUs; the same device for the in-process test
-// communicator) and polled by the consumer until the tag is the tag of this exchange
+// receiver's mailbox (xGMI peer store between GPUs; the same device for two processes on one GPU)
+// and polled by the consumer until the tag is the tag of this exchange
 // (MI355X_MICROARCH.md, hand-off price list: a granule needs no fence and no separate flag):
 //   tp_amax_quantize_kernel: row absmax of the local slice -> granule to every rank -> max of the
 //                            R granules -> Quantize of the slice with the global scale
@@ -25,6 +25,8 @@
 #include "kernels.h"
 #include "runtime.h"
 #include "tp_comm.h"
+
+#include <vector>
 
 namespace ct2x {
 
@@ -153,6 +155,16 @@ __global__ void tp_sum_epilogue_kernel(const void* __restrict__ partial, const f
   finish_exchange(ctl);
 }
 
+// One thread: says that it runs, waits until the other one does or `ticks` (of 10 ns) have passed.
+__global__ void tp_meet_kernel(uint32_t* mine, const uint32_t* other, uint32_t round, uint32_t* met, uint64_t ticks) {
+  __hip_atomic_store(mine, round, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  const uint64_t start = wall_clock64();
+  bool seen = false;
+  for (uint32_t spin = 0; spin < (1u << 20) && !seen && wall_clock64() - start < ticks; ++spin)
+    seen = __hip_atomic_load(other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) == round;
+  *met = seen ? 1u : 0u;
+}
+
 PeerBoxes boxes_of(const TpPeerBox& pb) {
   PeerBoxes p;
   for (int r = 0; r < kTpMaxWorld; ++r) p.box[r] = r < pb.world ? pb.box[r] : nullptr;
@@ -194,6 +206,47 @@ void launch_tp_sum_bias(const TpPeerBox& pb, const float* partial, const float* 
   hipLaunchKernelGGL((tp_sum_epilogue_kernel<false>), dim3(static_cast<unsigned>((total + 255) / 256)),
                      dim3(256), 0, stream, partial, nullptr, nullptr, bias, residual, n, total, y,
                      boxes_of(pb), pb.rank, pb.world);
+}
+
+void make_concurrent_streams(hipStream_t (&streams)[2]) {
+  constexpr int kTries = 8;
+  constexpr uint64_t kTicks = 1000000;  // 10 ms: far more than two launches take, and what a failed try costs
+  auto* words = static_cast<uint32_t*>(device_malloc(4 * sizeof(uint32_t)));  // the two's rounds, what they saw
+  std::vector<hipStream_t> made;
+  int partner = 0;
+  try {
+    CT2X_HIP_CHECK(hipMemset(words, 0, 4 * sizeof(uint32_t)));
+    CT2X_HIP_CHECK(hipDeviceSynchronize());
+    uint32_t round = 0;
+    for (int i = 0; i <= kTries && partner == 0; ++i) {
+      hipStream_t s = nullptr;
+      CT2X_HIP_CHECK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+      made.push_back(s);
+      // (a first launch on the stream, which meets itself: what is set up once is set up)
+      ++round;
+      hipLaunchKernelGGL(tp_meet_kernel, dim3(1), dim3(1), 0, s, words, words, round, words + 2, kTicks);
+      CT2X_HIP_CHECK(hipStreamSynchronize(s));
+      if (i == 0) continue;
+      ++round;
+      hipLaunchKernelGGL(tp_meet_kernel, dim3(1), dim3(1), 0, made[0], words, words + 1, round, words + 2, kTicks);
+      hipLaunchKernelGGL(tp_meet_kernel, dim3(1), dim3(1), 0, s, words + 1, words, round, words + 3, kTicks);
+      CT2X_HIP_CHECK(hipStreamSynchronize(made[0]));
+      CT2X_HIP_CHECK(hipStreamSynchronize(s));
+      uint32_t met[2];
+      CT2X_HIP_CHECK(hipMemcpy(met, words + 2, sizeof(met), hipMemcpyDeviceToHost));
+      if (met[0] && met[1]) partner = i;
+    }
+    CT2X_CHECK(partner != 0, "no two streams of this process run kernels at the same time");
+  } catch (...) {
+    for (hipStream_t s : made) (void)hipStreamDestroy(s);
+    device_free(words);
+    throw;
+  }
+  device_free(words);
+  streams[0] = made[0];
+  streams[1] = made[partner];
+  for (size_t i = 1; i < made.size(); ++i)
+    if (static_cast<int>(i) != partner) (void)hipStreamDestroy(made[i]);
 }
 
 }  // namespace ct2x

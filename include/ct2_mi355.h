@@ -790,7 +790,8 @@ void* ct2x_translator_create_tp_shm(const char* model_dir, int device_index, con
 int ct2x_tp_info(void* translator, int32_t* rank, int32_t* world, int32_t* has_mailboxes,
                  char* backend, int backend_size);
 /* The same sharded engines with an in-process communicator: `world` ranks in THIS process on ONE
- * device, each handle driven by its own host thread (the single-GPU test double of the above). */
+ * device, each handle driven by its own host thread (the single-GPU test double of the above; its
+ * collectives meet on the host, no kernel waits for another rank's). */
 /* Host-only: the rows of a column-parallel weight [n, k] owned by `rank` (Model::load,
  * src/models/model.cc:662-743). `blocks` are the sizes of the fused sub-matrices split separately
  * (Q | K | V); num_blocks = 0 means one block of n rows. first_out / count_out get one entry per
@@ -806,7 +807,8 @@ int ct2x_tp_selftest_local(int device_index, int world);
 /* The one-shot exchanges of a row-parallel int8 Dense (peer-mapped mailboxes, 8-byte {payload, tag}
  * granules stored and polled inside the producer / consumer kernels; SURVEY 8(e) "custom <= 1 MiB
  * one-shot path" instead of ops::ReduceAll, src/ops/nccl_ops_gpu.cu:53-68) on `world` in-process
- * ranks of one device: results checked bit for bit against the unsharded row, then `iters` exchange
+ * ranks of one device, on two streams that were seen to run at the same time (an error if no two of this
+ * process do): results checked bit for bit against the unsharded row, then `iters` exchange
  * pairs timed; *us_per_dense_out = microseconds per (absmax exchange + sum exchange), worst rank. */
 int ct2x_tp_selftest_oneshot(int device_index, int world, int64_t rows, int64_t depth, int64_t n,
                              int iters, float* us_per_dense_out);
