@@ -638,6 +638,9 @@ class Translator:  # also serves decoder-only models (ctranslate2.Generator) via
     def debug_inject_cluster_timeout(self):
         _lib.check(self._L.ct2x_debug_inject_cluster_timeout(C.c_void_p(self._h)))
 
+    def debug_give_up_exchanges(self):
+        _lib.check(self._L.ct2x_debug_give_up_exchanges(C.c_void_p(self._h)))
+
     def profile_begin(self):
         _lib.check(self._L.ct2x_profile_begin(C.c_void_p(self._h)))
 

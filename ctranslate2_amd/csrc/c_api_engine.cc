@@ -2109,6 +2109,15 @@ int ct2x_debug_inject_cluster_timeout(void* translator) {
   API_CATCH
 }
 
+int ct2x_debug_give_up_exchanges(void* translator) {
+  API_TRY
+  auto* t = static_cast<Translator*>(translator);
+  CT2X_CHECK(t != nullptr && t->engine, "ct2x_debug_give_up_exchanges: null translator");
+  CT2X_HIP_CHECK(hipSetDevice(t->engine->device_index()));
+  t->engine->debug_give_up_exchanges();
+  API_CATCH
+}
+
 int64_t ct2x_session_hits(void* translator) {
   auto* t = static_cast<Translator*>(translator);
   return t != nullptr ? t->session_hits : -1;

@@ -332,6 +332,10 @@ public:
   void enable_logits_history(DecodeState& state);
   void read_logits(DecodeState& state, int64_t first, int64_t count, float* out);
   void synchronize();
+  // Throws if a tensor-parallel exchange of this rank has given up (TpComm::check_exchanges): every way of
+  // results to the host passes here, check_cluster included.
+  void check_exchanges(DecodeState& state);
+  void debug_give_up_exchanges();
   // Throws ClusterTimeout if a cluster of the decoder-stack launch waited in vain for a member
   // during this session (something else held the compute units): its results are void. The
   // translate entry points catch it, switch the handle to the launch-per-op step

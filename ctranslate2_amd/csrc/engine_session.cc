@@ -435,7 +435,17 @@ void Engine::cluster_gate_release(int device_index) {
   g.held.store(false, std::memory_order_release);
 }
 
+void Engine::check_exchanges(DecodeState& st) {
+  if (tp_) tp_->check_exchanges(st.stream);
+}
+
+void Engine::debug_give_up_exchanges() {
+  CT2X_CHECK(tp_ != nullptr, "not a tensor-parallel rank");
+  tp_->debug_give_up();
+}
+
 void Engine::check_cluster(DecodeState& st) {
+  check_exchanges(st);
   if (st.cl_error == nullptr) return;
   if (st.cl_stamps != nullptr) {
     // phase timeline of workgroup 0 in the session's last step (wall_clock64: 100 MHz)
@@ -1107,6 +1117,7 @@ void Engine::prefill(DecodeState& st, const int32_t* h_ids, int64_t time, float*
   reset_lead_flags(st);
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
   check_last_launch("prefill");
+  if (logits_all) check_exchanges(st);
 }
 
 }  // namespace ct2x

@@ -846,6 +846,7 @@ void Engine::read_history(DecodeState& st, int64_t first, int64_t count, int32_t
                                   sizeof(float) * count * st.rows, hipMemcpyDeviceToHost,
                                   cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::read_history_async(DecodeState& st, int64_t first, int64_t count, int slot) {
@@ -888,6 +889,7 @@ void Engine::copy_logits_to_host(DecodeState& st, float* h_logits) {
   CT2X_HIP_CHECK(hipMemcpyAsync(h_logits, st.logits, sizeof(float) * st.rows * dec_.projection.n,
                                 hipMemcpyDeviceToHost, cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::set_ids(DecodeState& st, const int32_t* h_ids) {
@@ -1202,6 +1204,7 @@ void Engine::read_attention(DecodeState& st, int64_t first, int64_t count, float
   CT2X_HIP_CHECK(hipMemcpyAsync(out, st.att_hist + first * per_step, sizeof(float) * count * per_step,
                                 hipMemcpyDeviceToHost, cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::enable_logits_history(DecodeState& st) {
@@ -1226,6 +1229,7 @@ void Engine::read_logits(DecodeState& st, int64_t first, int64_t count, float* o
                                   st.logit_hist + ((first + s) % kLogitsRing) * per_step,
                                   sizeof(float) * per_step, hipMemcpyDeviceToHost, cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::set_step(DecodeState& st, int32_t step) {
@@ -1246,6 +1250,7 @@ void Engine::read_encoder_output(DecodeState& st, float* out) {
   CT2X_HIP_CHECK(hipMemcpyAsync(out, st.enc_out, sizeof(float) * st.batch * st.s_max * enc_.d_model,
                                 hipMemcpyDeviceToHost, cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::set_whisper_processing(DecodeState& st, const WhisperProcessing& wp) {
@@ -1368,6 +1373,7 @@ void Engine::read_no_speech_probs(DecodeState& st, float* out) {
   CT2X_HIP_CHECK(hipMemcpyAsync(out, st.d_no_speech, sizeof(float) * st.rows, hipMemcpyDeviceToHost,
                                 cur_stream()));
   CT2X_HIP_CHECK(hipStreamSynchronize(cur_stream()));
+  check_exchanges(st);
 }
 
 void Engine::score_targets(DecodeState& st, const int32_t* h_inputs, const int32_t* h_outputs,

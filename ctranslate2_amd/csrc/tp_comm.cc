@@ -11,6 +11,7 @@
 #include <atomic>
 #include <chrono>
 #include <condition_variable>
+#include <cstddef>
 #include <thread>
 #include <cstdlib>
 #include <cstring>
@@ -21,6 +22,26 @@
 #include "runtime.h"
 
 namespace ct2x {
+
+void TpComm::check_exchanges(hipStream_t stream) const {
+  const TpPeerBox* pb = peer_box();
+  if (pb == nullptr) return;
+  uint32_t status = 0;
+  CT2X_HIP_CHECK(hipMemcpyAsync(&status, pb->box[pb->rank] + offsetof(TpBoxControl, status), sizeof(status),
+                                hipMemcpyDeviceToHost, stream));
+  CT2X_HIP_CHECK(hipStreamSynchronize(stream));
+  if (status != 0)
+    throw Error("tensor parallel exchange: a rank did not arrive within the bounded wait of rank " +
+                std::to_string(pb->rank) + "; the results are void, create the ranks anew");
+}
+
+void TpComm::debug_give_up() const {
+  const TpPeerBox* pb = peer_box();
+  if (pb == nullptr) throw Error("this communicator has no mailboxes");
+  const uint32_t status = 1;
+  CT2X_HIP_CHECK(hipMemcpy(pb->box[pb->rank] + offsetof(TpBoxControl, status), &status, sizeof(status),
+                           hipMemcpyHostToDevice));
+}
 
 // ---------------------------------------------------------------------------------------------
 // RCCL over xGMI. The library is resolved at run time: the single-GPU product path must load on

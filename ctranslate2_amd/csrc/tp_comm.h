@@ -57,6 +57,13 @@ public:
   // Mailboxes for the one-shot exchanges, or nullptr when this communicator has none (the engine
   // then uses the collectives below).
   virtual const TpPeerBox* peer_box() const { return nullptr; }
+  // Waits for `stream` and throws if a poll of this rank's one-shot exchanges has ever given up: zeros
+  // stand in the place of a peer's values then, here and (fail fast) in every exchange that follows, so
+  // whatever was computed is void and the communicator is of no more use. Called wherever results of
+  // exchanges reach the host. Nothing to do without mailboxes.
+  void check_exchanges(hipStream_t stream) const;
+  // Tests: marks this rank's mailbox as if a poll had given up.
+  void debug_give_up() const;
   virtual int rank() const = 0;
   virtual int world() const = 0;
   // In-place all-reduce of `count` elements at `buf` (device memory of this rank) on `stream`.

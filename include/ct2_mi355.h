@@ -1006,6 +1006,12 @@ int64_t ct2x_cluster_fallbacks(void* translator);
 int ct2x_debug_inject_cluster_timeout(void* translator);
 int ct2x_release_session(void* translator);
 
+/* The one-shot exchanges of tensor-parallel ranks wait in their kernels, bounded: a rank that does not
+ * arrive within some seconds is given up, zeros stand for its values, and every call that hands results to
+ * the host fails from then on (the ranks have to be created anew). ct2x_debug_give_up_exchanges (tests):
+ * marks this rank as if that had happened; on every rank, before a call. */
+int ct2x_debug_give_up_exchanges(void* translator);
+
 /* Per-kernel profile of the next translate/generate calls, measured with HIP events on the
  * engine's stream around every launch (graph replay is disabled while profiling). profile_end
  * writes a JSON object {label: {"launches":n,"total_ms":t,"bytes":b,"ops":o}, ...} where bytes /

@@ -61,3 +61,61 @@ def test_one_shot_exchanges_beside_many_streams(gpu):
     _lib.check(_lib.lib().ct2x_tp_selftest_oneshot(0, 2, C.c_int64(32), C.c_int64(256), C.c_int64(512), 20,
                                                    C.byref(us)))
     assert us.value > 0
+
+
+RANK = """
+import json, sys
+import numpy as np
+import ctranslate2_amd as ct2
+model, rank, segment, sources, steps = sys.argv[1], int(sys.argv[2]), sys.argv[3], json.loads(sys.argv[4]), 4
+t = ct2.Translator.tensor_parallel_shm(model, rank, 2, segment, compute_type="int8")
+kw = dict(beam_size=2, max_decoding_length=8, min_decoding_length=8)
+tgt = np.ones((len(sources), steps), np.int32)
+same = [s[:1] for s in sources]
+t.translate_ids(sources, **kw)
+t.step_logits(same, tgt)
+t.debug_give_up_exchanges()
+errors = []
+for call in (lambda: t.translate_ids(sources, **kw), lambda: t.translate_ids(sources, beam_size=1, **{
+        k: v for k, v in kw.items() if k != "beam_size"}), lambda: t.step_logits(same, tgt)):
+    try:
+        call()
+        errors.append("")
+    except ct2.Ct2xError as e:
+        errors.append(str(e))
+print("ERRORS " + json.dumps(errors))
+t.close()
+"""
+
+
+def test_a_wait_in_vain_is_an_error(gpu):
+    """A poll that gave up (marked by the host on both ranks, so that no kernel waits) makes every call that hands
+    out results fail: greedy and beam search, logits."""
+    import json
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    segment = "ct2x_tp_give_up_%d" % os.getpid()
+    env = dict(os.environ, HSA_ENABLE_IPC_MODE_LEGACY="0", PYTHONPATH=root)
+    procs = [subprocess.Popen([sys.executable, "-c", RANK, _model_dir("tiny"), str(r), segment,
+                               json.dumps(_sources("tiny"))], env=env, cwd=root, stdout=subprocess.PIPE,
+                              stderr=subprocess.PIPE, text=True) for r in range(2)]
+    try:
+        outs = [p.communicate(timeout=60) for p in procs]
+    finally:
+        for p in procs:
+            p.kill()
+    for p, (out, err) in zip(procs, outs):
+        assert p.returncode == 0, err[-2000:]
+        errors = json.loads(next(line for line in out.splitlines() if line.startswith("ERRORS "))[7:])
+        assert len(errors) == 3 and all("did not arrive" in e for e in errors), errors
+
+
+def test_give_up_needs_mailboxes(gpu):
+    import ctranslate2_amd as ct2
+    path = _model_dir("tiny")
+    for t in [ct2.Translator(path)] + ct2.Translator.tensor_parallel_local(path, 2):
+        with pytest.raises(ct2.Ct2xError, match="tensor-parallel rank|no mailboxes"):
+            t.debug_give_up_exchanges()
+        t.close()
