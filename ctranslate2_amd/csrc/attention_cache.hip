@@ -44,6 +44,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "cache_line.h"
 #include "cache_ops.h"
 #include "device_utils.h"
 #include "runtime.h"
@@ -119,18 +120,6 @@ __device__ __forceinline__ int rounds_of(const CacheAttnParams& p, const CachePl
   const int n = (walked(p, b) + (1 << plan.round_shift) - 1) >> plan.round_shift;
   return n < 1 ? 1 : n;
 }
-
-// The line of all rounds and how many workgroups share it: the first `longer` take `each` + 1 rounds.
-// (A line has less than 2048 units - launch_cache_attention - of at most 2^20 rounds.)
-struct Line {
-  uint32_t total, groups, each, longer;
-  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * each + (w < longer ? w : longer); }
-  // the workgroup that holds round x
-  __device__ __forceinline__ uint32_t holder(uint32_t x) const {
-    const uint32_t ahead = longer * (each + 1);
-    return x < ahead ? x / (each + 1) : longer + (x - ahead) / each;
-  }
-};
 
 // ---- the types -------------------------------------------------------------------------------
 
@@ -829,12 +818,10 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
   const uint32_t units = static_cast<uint32_t>(p.heads_kv) * plan.row_groups;
   Line line{0, 0, 1, 0};
   int64_t b = 0;
-  uint32_t before = 0, x, x1;  // the round of the line that entry b begins at, the workgroup's stretch
-  if (plan.whole) {  // a line of the one entry
+  Stretch stretch{0, 0, 0, 0};
+  if (plan.whole) {
     b = blockIdx.x / units;
-    const uint32_t n = uniform(rounds_of(p, plan, b));
-    x = blockIdx.x % units * n;
-    x1 = x + n;
+    stretch = Stretch::whole(blockIdx.x % units, uniform(rounds_of(p, plan, b)));
   } else {
     const int lane = threadIdx.x & 63;
     auto rounds = [&](int64_t entry) {
@@ -851,15 +838,16 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
     line.each = line.total / line.groups;
     line.longer = line.total - line.each * line.groups;
     if (blockIdx.x >= line.groups) return;
-    x = line.start(blockIdx.x);
-    x1 = line.start(blockIdx.x + 1);
-    // the entry that x lies in
+    stretch.x = line.start(blockIdx.x);
+    stretch.x1 = line.start(blockIdx.x + 1);
+    // the entry that the stretch begins in
+    uint32_t before = 0;
     for (;; b += 64) {
       if (p.batch > 64) {
         mine = rounds(b + lane);
         upto = wave_scan(mine);
       }
-      const uint64_t behind = __ballot(before + upto > x);
+      const uint64_t behind = __ballot(before + upto > stretch.x);
       if (behind) {
         const int at = __builtin_ctzll(behind);
         before += __builtin_amdgcn_readlane(upto - mine, at);
@@ -868,27 +856,23 @@ void cache_attention_kernel(CacheAttnParams p, CachePlan plan) {
       }
       before += __builtin_amdgcn_readlane(upto, 63);
     }
+    stretch.before = before;
   }
-  const uint32_t x0 = x;
+  const uint32_t x0 = stretch.x;
 #pragma unroll 1
-  while (x < x1) {
+  while (stretch.x < stretch.x1) {
     const uint32_t n = uniform(rounds_of(p, plan, b));
-    const uint32_t unit = (x - before) / n, r0 = x - before - unit * n;
-    const uint32_t r1 = x1 - x < n - r0 ? r0 + (x1 - x) : n;
-    worker.begin(b, unit, r0, r1);
-    worker.walk(r0, r1);
+    const Stretch::Part part = stretch.part(n);
+    worker.begin(b, part.unit, part.r0, part.r1);
+    worker.walk(part.r0, part.r1);
     // a part that begins the workgroup's stretch is its first, any other its last
-    const int slot = blockIdx.x * 2 + (x == x0 ? 0 : 1);
-    if (!plan.whole && r0 == 0 && threadIdx.x == 0) {
-      const int count = static_cast<int>(line.holder(x + n - 1) - blockIdx.x) + 1;
-      reinterpret_cast<int2*>(static_cast<float*>(p.scratch) + plan.records)[b * units + unit] = int2{slot, count};
+    const int slot = blockIdx.x * 2 + (stretch.x == x0 ? 0 : 1);
+    if (!plan.whole && part.r0 == 0 && threadIdx.x == 0) {
+      const int count = static_cast<int>(line.holder(stretch.x + n - 1) - blockIdx.x) + 1;
+      reinterpret_cast<int2*>(static_cast<float*>(p.scratch) + plan.records)[b * units + part.unit] = int2{slot, count};
     }
-    worker.finish(r0 == 0 && r1 == n, slot);
-    x += r1 - r0;
-    if (x == before + n * units) {
-      before = x;
-      ++b;
-    }
+    worker.finish(part.r0 == 0 && part.r1 == n, slot);
+    if (stretch.pass(part, n, units)) ++b;
   }
 }
 
@@ -1076,7 +1060,8 @@ CachePlan make_plan(const CacheAttnParams& p) {
   static constexpr int kAlone[3][3] = {{2, 8, 16}, {2, 4, 32}, {8, 16, 32}};
   const int many = units >= 512 ? 2 : units >= 192 ? 1 : 0;
   const int view = p.view == CacheView::kDense ? 0 : p.view == CacheView::kBlocks ? 1 : 2;
-  plan.whole = walked <= round_keys * kAlone[view][many] || units >= 2048;
+  plan.whole = walked <= round_keys * kAlone[view][many] || units >= 2048 ||
+               line_is_too_long(units, (walked + round_keys - 1) / round_keys);
   // scratch
   auto up = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   const int64_t parts = plan.whole ? 0 : 2ll * plan.grid * plan.unit_rows;
