@@ -71,6 +71,16 @@ void check_alignment(const char* name, const P*... pointers) {
     CACHE_CHECK(reinterpret_cast<uintptr_t>(p) % 16 == 0, "tensors must be aligned to 16 bytes");
 }
 
+// The bytes that an argument covers.
+struct Span {
+  const void* at;
+  int64_t bytes;
+  bool apart(const Span& other) const {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(at), y = reinterpret_cast<uintptr_t>(other.at);
+    return bytes == 0 || other.bytes == 0 || x + bytes <= y || y + other.bytes <= x;
+  }
+};
+
 void check_scratch(const char* name, const void* d_scratch, int64_t bytes, int64_t need) {
   CACHE_CHECK(need == 0 || (d_scratch != nullptr && bytes >= need),
               "scratch missing or smaller than the _scratch_bytes() function says");
@@ -221,22 +231,21 @@ int ct2x_cache_evict(const void* d_k_cache, const void* d_v_cache, int kv_dtype,
   if (batch == 0) return 0;
   check_pointers(name, d_k_cache, d_v_cache, d_weights, d_k_out, d_v_out, d_weights_out, d_positions, d_lengths_out);
   check_alignment(name, d_k_cache, d_v_cache, d_k_out, d_v_out);
-  // in place, or nowhere near: an output that overlaps its input another way would be read after it
-  // was overwritten
+  // in place, or nowhere near: what one workgroup writes, another may still have to read
   const int64_t row = dhead * element_bytes(kv_dtype), in = batch * heads_kv * t_max, out = batch * heads_kv * t_max_out;
-  auto apart = [&](const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x + a_bytes <= y || y + b_bytes <= x;
-  };
-  auto in_place_or_apart = [&](const void* a, const void* b, int64_t unit) {
-    return (a == b && t_max == t_max_out) || apart(a, in * unit, b, out * unit);
-  };
-  CACHE_CHECK(in_place_or_apart(d_k_cache, d_k_out, row) && in_place_or_apart(d_v_cache, d_v_out, row) &&
-                  in_place_or_apart(d_weights, d_weights_out, 4),
-              "an output must be its input (same t_max) or not overlap it");
-  CACHE_CHECK(apart(d_k_out, out * row, d_v_cache, in * row) && apart(d_v_out, out * row, d_k_cache, in * row) &&
-                  apart(d_k_out, out * row, d_v_out, out * row),
-              "keys and values overlap");
+  const Span inputs[] = {{d_k_cache, in * row}, {d_v_cache, in * row}, {d_weights, in * 4},
+                         {d_lengths, d_lengths ? batch * 4 : 0}};
+  const Span outputs[] = {{d_k_out, out * row}, {d_v_out, out * row}, {d_weights_out, out * 4},
+                          {d_lengths_out, batch * 4}, {d_positions, batch * heads_kv * budget * 4}};
+  for (int o = 0; o < 5; ++o) {
+    for (int i = 0; i < 4; ++i) {
+      // an output's own input: the first three with the same room, the lengths always
+      const bool in_place = o == i && outputs[o].at == inputs[i].at && (o == 3 || t_max == t_max_out);
+      CACHE_CHECK(in_place || outputs[o].apart(inputs[i]),
+                  "outputs and inputs overlap (an output may be its own input, with the same t_max)");
+    }
+    for (int i = 0; i < o; ++i) CACHE_CHECK(outputs[o].apart(outputs[i]), "two outputs overlap");
+  }
   CacheEvictParams p;
   p.k = d_k_cache;
   p.v = d_v_cache;

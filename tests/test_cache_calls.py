@@ -3,7 +3,7 @@ checks refuse beyond tests/test_cache_refusals.py. No GPU: every call ends in th
 import pytest
 
 from ctranslate2_amd import _lib
-from test_cache_refusals import S, evict, refused
+from test_cache_refusals import A, B, C, D, E, S, evict, refused
 
 
 def test_eviction_takes_the_tail_of_the_attention_calls():
@@ -36,3 +36,34 @@ def test_eviction_refuses_other_numbers_of_arguments(change):
     own = evict(batch=0)[1]
     with pytest.raises(TypeError, match="arguments"):
         _lib.lib().ct2x_cache_evict(*(own[:change] if change < 0 else own + [None] * change))
+
+
+# the arguments of `evict` by where they lie: k A, v B, weights C, k_out D, v_out E, weights_out S,
+# positions S + 4096, lengths_out S + 8192; keys and values in are 4096 bytes, out 1024, weights in 128, out 32,
+# positions 32, lengths 4
+@pytest.mark.parametrize("change", [
+    dict(weights_out=A), dict(weights_out=B + 4064), dict(weights_out=D + 512), dict(weights_out=E),
+    dict(weights_out=C + 64), dict(weights_out=C), dict(positions=A + 4092), dict(positions=B), dict(positions=C),
+    dict(positions=C + 124), dict(positions=D), dict(positions=E + 1020), dict(positions=S), dict(positions=S + 28),
+    dict(lengths_out=A), dict(lengths_out=B + 4092), dict(lengths_out=C + 4), dict(lengths_out=D), dict(lengths_out=E),
+    dict(lengths_out=S + 28), dict(lengths_out=S + 4096 + 28),
+    dict(k_out=C - 1008), dict(v_out=C + 112), dict(k_out=B), dict(k_out=A, t_max_out=8), dict(v_out=B, t_max_out=8),
+    # two entries' lengths on the device: one entry apart is an overlap, the same pointer is in place
+    dict(batch=2, lengths=S + 16384, lengths_out=S + 16388), dict(batch=2, lengths=S + 16388, lengths_out=S + 16384),
+    dict(lengths=S + 16384, positions=S + 16380), dict(lengths=S + 16384, weights_out=S + 16384),
+    dict(lengths=D + 64), dict(lengths=E + 1020),
+], ids=str)
+def test_eviction_refuses_every_other_overlap(change):
+    assert "overlap" in refused(*evict(**change))
+
+
+def test_eviction_in_place_passes_the_overlap_checks():
+    """What follows the overlap checks is a launch: the checks are passed where the error is not theirs (no GPU) or
+    there is none to be had without one."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are numbers")
+    for change in (dict(), dict(k_out=A, v_out=B, weights_out=C, t_max_out=16), dict(v_out=B, t_max_out=16),
+                   dict(lengths=S + 8192), dict(lengths=S + 16384, positions=S + 16384 - 32), dict(k_out=A + 4096),
+                   dict(lengths_out=C + 128), dict(positions=S + 32)):
+        assert "overlap" not in refused(*evict(**change)), change
