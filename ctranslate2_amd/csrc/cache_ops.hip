@@ -17,6 +17,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSelectThreads = 1024;
+// A launch has less than 2^32 threads: more rows - (entry, head of the cache) pairs - take several launches.
+constexpr int64_t kMostGroups = int64_t{1} << 21;
 
 __device__ __forceinline__ uint32_t order_key(float x) {
   if (x != x) return 0xfffffffeu;
@@ -222,8 +224,8 @@ __device__ int emit_selected(const Keys<K, F>& keys, K threshold, int ties, G em
 
 // positions[b, hkv, :]: what stays, ascending, -1 behind the last. One workgroup per row: bound by the
 // latency of its passes (64 rows of 16 k weights: 16 us; histograms split by lane took the same).
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvictParams p) {
-  const int64_t row = blockIdx.x, b = row / p.heads_kv;
+__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvictParams p, int64_t row0) {
+  const int64_t row = row0 + blockIdx.x, b = row / p.heads_kv;
   const int n = static_cast<int>(clamped_length(p.lengths, p.length, b, p.t_max));
   const int budget = static_cast<int>(p.budget), recent = static_cast<int>(p.recent);
   const float* w = p.weights + row * p.t_max;
@@ -247,11 +249,11 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(CacheEvict
 // turn may write where it reads. Apart, `chunks` workgroups take the steps. Bound by the copy: 64 rows of
 // 4096 kept positions of 128 bfloat16 apart 56 us, 4.8 TB/s.
 constexpr int kMoveThreads = 512, kMoveSteps = 4;
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(CacheEvictParams p, int row_bytes, int slices,
-                                                                  int chunks) {
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(CacheEvictParams p, int64_t row0, int row_bytes,
+                                                                  int slices, int chunks) {
   constexpr int kRows = kMoveThreads / 8;
   const int chunk = blockIdx.x % chunks, part = blockIdx.x / chunks % (2 * slices);
-  const int64_t row = blockIdx.x / chunks / (2 * slices), b = row / p.heads_kv;
+  const int64_t row = row0 + blockIdx.x / chunks / (2 * slices), b = row / p.heads_kv;
   const int slice = part >> 1, value = part & 1;
   const int32_t* positions = p.positions + row * p.budget;
   const char* from = static_cast<const char*>(value ? p.v : p.k) + row * p.t_max * row_bytes;
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(CacheEvictPara
       if (t[i] >= 0 && weighs) w_out[j] = weight[i];
     }
   }
-  if (blockIdx.x % (2 * slices * chunks * p.heads_kv) == 0 && threadIdx.x == 0) {
+  if (chunk == 0 && part == 0 && row == b * p.heads_kv && threadIdx.x == 0) {
     const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
     p.lengths_out[b] = static_cast<int32_t>(n < p.budget ? n : p.budget);
   }
@@ -516,8 +518,8 @@ __global__ __launch_bounds__(kThreads) void block_scores_kernel(CacheSelectParam
   }
 }
 
-__global__ __launch_bounds__(kSelectThreads) void block_select_kernel(CacheSelectParams p, int64_t blocks) {
-  const int64_t row = blockIdx.x, b = row / p.heads_kv;
+__global__ __launch_bounds__(kSelectThreads) void block_select_kernel(CacheSelectParams p, int64_t row0, int64_t blocks) {
+  const int64_t row = row0 + blockIdx.x, b = row / p.heads_kv;
   const int64_t n = clamped_length(p.lengths, p.length, b, p.t_max);
   const int count = static_cast<int>((n + p.block - 1) / p.block), top = static_cast<int>(p.top);
   const double* scores = p.scores + row * blocks;
@@ -537,6 +539,14 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(CacheSelec
 int walkers_for(int64_t rows, int64_t pieces) {
   const int64_t fill = (2048 + rows - 1) / rows;
   return static_cast<int>(fill < pieces ? fill : pieces);
+}
+
+// launch(first row, workgroups) for stretches of rows with `per_row` workgroups each
+template <typename F>
+void for_rows(int64_t rows, int64_t per_row, F launch) {
+  const int64_t most = kMostGroups / per_row;
+  for (int64_t row0 = 0; row0 < rows; row0 += most)
+    launch(row0, static_cast<unsigned>((rows - row0 < most ? rows - row0 : most) * per_row));
 }
 
 template <typename T>
@@ -566,9 +576,13 @@ void launch_cache_evict(const CacheEvictParams& p, hipStream_t stream) {
   const int64_t steps = (p.budget + kMoveThreads / 8 * kMoveSteps - 1) / (kMoveThreads / 8 * kMoveSteps);
   // in place the steps have an order
   const int chunks = p.k == p.k_out || p.v == p.v_out || p.weights == p.weights_out ? 1 : walkers_for(rows * 2 * slices, steps);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, stream, p);
-  hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(rows * 2 * slices * chunks)), dim3(kMoveThreads), 0,
-                     stream, p, row_bytes, slices, chunks);
+  for_rows(rows, 1, [&](int64_t row0, unsigned groups) {
+    hipLaunchKernelGGL(evict_select_kernel, dim3(groups), dim3(kSelectThreads), 0, stream, p, row0);
+  });
+  for_rows(rows, 2 * slices * chunks, [&](int64_t row0, unsigned groups) {
+    hipLaunchKernelGGL(evict_move_kernel, dim3(groups), dim3(kMoveThreads), 0, stream, p, row0, row_bytes, slices,
+                       chunks);
+  });
 }
 
 void launch_cache_block_bounds(const CacheBoundsParams& p, hipStream_t stream) {
@@ -583,8 +597,9 @@ void launch_cache_select(const CacheSelectParams& p, hipStream_t stream) {
   if (p.kv_dtype == 0) scores_typed<float>(p, blocks, stream);
   else if (p.kv_dtype == 4) scores_typed<__half>(p, blocks, stream);
   else scores_typed<uint16_t>(p, blocks, stream);
-  hipLaunchKernelGGL(block_select_kernel, dim3(static_cast<unsigned>(p.batch * p.heads_kv)), dim3(kSelectThreads),
-                     0, stream, p, blocks);
+  for_rows(p.batch * p.heads_kv, 1, [&](int64_t row0, unsigned groups) {
+    hipLaunchKernelGGL(block_select_kernel, dim3(groups), dim3(kSelectThreads), 0, stream, p, row0, blocks);
+  });
 }
 
 }  // namespace ct2x

@@ -537,7 +537,8 @@ int ct2x_attention_full_half(const float* d_q, const float* d_k, const float* d_
  * All of them work on K / V caches [batch, heads_kv, t_max, dhead] of kv_dtype (CT2X_F32 / CT2X_F16 /
  * CT2X_BF16; values as raw 2-byte data) with fp32 queries and outputs. dhead is a multiple of 8 up to
  * 256, heads a multiple of heads_kv (head h reads head h / (heads / heads_kv) of the cache), t_max *
- * dhead * 4 <= 2^31 - 2^20; tensors are aligned to 16 bytes. Entry b has d_lengths[b] committed positions
+ * dhead * 4 <= 2^31 - 2^20, batch * heads_kv <= 2^22, heads / heads_kv <= 1024, batch * tokens * heads <=
+ * 2^26; tensors are aligned to 16 bytes. Entry b has d_lengths[b] committed positions
  * (clamped to what the cache holds), or `length` where d_lengths is NULL (`length` is not read
  * otherwise). What lies behind an entry's positions is never looked at: it may hold anything.
  * Scores, softmax statistics and sums are fp32. Products with 16-bit caches run on the 16-bit matrix

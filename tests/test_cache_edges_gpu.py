@@ -38,3 +38,52 @@ def test_tree_committed_values_that_are_not_finite(gpu, dtype, tokens, heads, dh
         v[0, 0, at, channel] = held
     got = C.run_tree(q, k, v, dtype, None, n, C.to_words(seen), scale)
     C.check_tree(got, q, k, v, dtype, [n], seen, scale)
+
+
+ROWS = 2 ** 22  # the most (entry, head of the cache) pairs of a call
+
+
+def test_evict_of_the_most_rows(gpu):
+    """A launch holds less than 2^32 threads: this many rows take several."""
+    gen = C.generator(42)
+    shape = (ROWS // 2, 2, 2, 8)
+    k = torch.randn(shape, device="cuda", generator=gen).half()
+    v = torch.randn(shape, device="cuda", generator=gen).half()
+    w = torch.rand(shape[:3], device="cuda", generator=gen)
+    k_out, v_out, w_out = k[:, :, :1].clone(), v[:, :, :1].clone(), w[:, :, :1].clone()
+    n_out = torch.full((shape[0],), -7, dtype=torch.int32, device="cuda")
+    positions = C.run_evict(k, v, w, "f16", None, 2, 1, 0, k_out, v_out, w_out, n_out)
+    heavier = (w[:, :, 1] > w[:, :, 0]).int()
+    assert torch.equal(positions[:, :, 0], heavier)
+    at = heavier.long()[:, :, None]
+    assert torch.equal(w_out, torch.gather(w, 2, at))
+    for out, old in ((k_out, k), (v_out, v)):
+        assert torch.equal(out, torch.gather(old, 2, at[..., None].expand(-1, -1, -1, 8)))
+    assert bool((n_out == 1).all())
+
+
+def test_blocks_of_the_most_rows(gpu):
+    gen = C.generator(43)
+    batch, t_max = ROWS // 2, 17
+    shape = (batch, 2, t_max, 8)
+    k = torch.randn(shape, device="cuda", generator=gen).half()
+    v = torch.randn(shape, device="cuda", generator=gen).half()
+    q = torch.randn((batch, 2, 8), device="cuda", generator=gen)
+    out, selected = torch.full_like(q, 7.0), torch.full((batch, 2, 1), 7, dtype=torch.int32, device="cuda")
+    bounds = torch.zeros((batch, 2, 2, 2, 8), dtype=k.dtype, device="cuda")
+    L = _lib.lib()
+    need = L.ct2x_attention_blocks_scratch_bytes(batch, 2, 2, 8, t_max, 16, 1)
+    scratch = torch.empty((need,), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    _lib.check(L.ct2x_cache_block_bounds(_lib.ptr(k), 4, None, None, t_max, batch, 2, 8, t_max, 16, _lib.ptr(bounds),
+                                         None))
+    _lib.check(L.ct2x_attention_blocks(
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), 4, _lib.ptr(bounds), None, t_max, batch, 2, 2, 8, t_max, 16, 1, 0, 1,
+        0.3, _lib.ptr(out), _lib.ptr(selected), _lib.ptr(scratch), need, None))
+    C.sync()
+    assert bool((selected == 1).all())  # the last block, of one position: its value
+    assert torch.equal(bounds[:, :, 1, 0], k[:, :, 16]) and torch.equal(bounds[:, :, 0, 1], k[:, :, :16].amax(2))
+    # One probability p, whatever its reference: out = (y0 v + y1 v) (1 / p) with y0 + y1 within 2^-22 of p; the sum,
+    # the reciprocal (2^-23 allowed) and the last product round by 2^-24 each: 2^-21 in all.
+    want = v[:, :, 16].double()
+    assert bool(((out.double() - want).abs() <= 2.0 ** -21 * want.abs()).all())
