@@ -31,7 +31,14 @@
 // the transposing LDS read instead of v_perm 220 against 207.
 //
 // 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as a sum of
-// 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-11 (float16).
+// 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-12 (float16).
+// Three of bfloat16 leave 2^-27. float16's steps end at 2^-24, so that a second term of something small holds
+// only its first bits. A query's is therefore what the first left times 2^11, with sums of its own that
+// join the others' times 2^-11: 2^-22 of an element is left, or 2^-36 of the row's largest (unscaled: 2^-25 of the
+// row's largest; 300 positions, one query channel of 16384 beside others of 2: outputs off by 4e-4). A
+// probability's range ends below 2^16 and begins at 2^13 (kLift): 2^-22 of it is left, or 2^-38 of the row's
+// largest. (Sums of their own for it as well: 5 to 15 % of a tree's time, 340 for 290 us on 16 x 64 tokens and
+// 8 k positions.)
 // float32 caches use the float32 MFMA, nothing is rounded.
 //
 // Work is cut evenly whatever the lengths: the rounds (kStep positions per wave that shares a row
@@ -132,16 +139,17 @@ struct Mfma {  // 16-bit
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
                                                      0);
   }
-  // the pair x0, x1 as a sum of kTerms pairs of 16-bit values, up to half a step of the last
+  // the pair x0, x1 as a sum of kTerms pairs of 16-bit values, up to half a step of the last, each after the
+  // first times 1 / back
   template <int kTerms>
-  static __device__ __forceinline__ void split(float x0, float x1, uint32_t (&terms)[kTerms]) {
+  static __device__ __forceinline__ void split(float x0, float x1, uint32_t (&terms)[kTerms], float back = 1.f) {
     v2f x = {x0, x1};
 #pragma unroll
     for (int t = 0; t < kTerms; ++t) {
       if constexpr (kType == kF16) {
         const v2h y = __builtin_convertvector(x, v2h);
         terms[t] = __builtin_bit_cast(uint32_t, y);
-        x -= __builtin_convertvector(y, v2f);
+        x = (x - __builtin_convertvector(y, v2f)) * (1.f / back);
       } else {
         const v2bf y = __builtin_convertvector(x, v2bf);
         terms[t] = __builtin_bit_cast(uint32_t, y);
@@ -221,10 +229,12 @@ struct Worker {
   // bfloat16 (2^-18) and 32 rows a wave took 200 us where 16 rows and three take 305 (4 entries of 23 k, 64
   // tokens), with an error twice that of float32 arithmetic (4.6e-6): not taken.
   static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 ? 3 : 2;
+  static constexpr bool kApart = kType == kF16;  // the products of the queries' second terms have sums of their own
+  static constexpr float kBack = kApart ? 1.f / 2048 : 1.f;  // and this factor
   uint32_t queries[kTerms][NT][T::kChunks][4];
   // Probabilities are 2^(s + kLift - reference): the reference is a maximum that later ones exceed by up to
-  // kSlack, so that outputs are rescaled seldom, and float16, whose steps end at 2^-24, takes them 2^6 larger.
-  static constexpr float kSlack = 8.f, kLift = kType == kF16 ? 6.f : 0.f;
+  // kSlack, so that outputs are rescaled seldom. float16 ends below 2^16, its steps at 2^-24: 2^15 at most.
+  static constexpr float kSlack = kType == kF16 ? 2.f : 8.f, kLift = kType == kF16 ? 13.f : 0.f;
   float factor[NT];  // > 0: scores are factor times what the matrix cores give, to the base 2
   float m[NT], l[NT];  // m: without the factor until the walk ends
   v4f o[NT][T::E];
@@ -336,7 +346,7 @@ struct Worker {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t terms[kTerms];
-            Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, terms);
+            Mfma<kType>::split(x[s][2 * j] * down, x[s][2 * j + 1] * down, terms, kBack);
 #pragma unroll
             for (int t = 0; t < kTerms; ++t) queries[t][n][s][j] = terms[t];
           }
@@ -493,11 +503,11 @@ struct Worker {
     if constexpr (kShared) __builtin_amdgcn_s_setprio(1);
     float s[NT][T::kLane];
     {
-      v4f acc[NT][T::kKeyTiles];
+      v4f acc[NT][T::kKeyTiles], acc_low[NT][T::kKeyTiles];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < T::kKeyTiles; ++i) acc[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < T::kKeyTiles; ++i) acc[n][i] = acc_low[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
       // (independent products follow each other: a product waits for the one that it adds to)
 #pragma unroll
       for (int x = 0; x < T::kChunks; ++x)
@@ -507,9 +517,11 @@ struct Worker {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int i = 0; i < T::kKeyTiles; ++i)
-                acc[n][i] = Mfma<kType>::mul(k[i][x], v4u{queries[t][n][x][0], queries[t][n][x][1], queries[t][n][x][2], queries[t][n][x][3]},
-                                             acc[n][i]);
+              for (int i = 0; i < T::kKeyTiles; ++i) {
+                const v4u q = {queries[t][n][x][0], queries[t][n][x][1], queries[t][n][x][2], queries[t][n][x][3]};
+                v4f& to = kApart && t == 1 ? acc_low[n][i] : acc[n][i];
+                to = Mfma<kType>::mul(k[i][x], q, to);
+              }
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -521,7 +533,10 @@ struct Worker {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < T::kLane; ++j) s[n][j] = acc[n][j / 4][j % 4];
+        for (int j = 0; j < T::kLane; ++j) {
+          s[n][j] = acc[n][j / 4][j % 4];
+          if constexpr (kApart) s[n][j] = fmaf(acc_low[n][j / 4][j % 4], kBack, s[n][j]);
+        }
     }
     if constexpr (kShared) {
       __builtin_amdgcn_s_setprio(0);
@@ -1030,8 +1045,8 @@ CachePlan make_plan(const CacheAttnParams& p) {
   const int waves = waves_of(plan.shared);
   // 32 rows a wave read the tiles half as often, 16 have a shorter way in and out: the former where there are
   // rows for eight such waves and enough positions times rows. float16, heads of 128, 64 tokens, us by 16 / 32:
-  // 4 entries of 500 30.7 / 42.9, 4 of 2000 48 / 59, 4 of 8000 107 / 103, 16 of 8000 356 / 306; float32 51 / 70,
-  // 104 / 119, 314 / 313, 1139 / 1060. Three bfloat16 terms of 32 rows of 128 channels are more than the
+  // 4 entries of 500 32 / 46, 4 of 2000 50 / 64, 4 of 8000 103 / 107, 16 of 8000 340 / 298; float32 51 / 69,
+  // 104 / 113, 301 / 296, 1135 / 1045. Three bfloat16 terms of 32 rows of 128 channels are more than the
   // registers: 16 of 8000 take 414 us by 16, 518 by 32.
   const bool long_tree = rows > 128 && rows * p.t_max * p.heads_kv * p.batch >= 60000000;
   plan.tiles = plan.shared && long_tree && (p.kv_dtype != kBF16 || dp <= 64) ? 2 : 1;

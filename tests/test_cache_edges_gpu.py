@@ -87,3 +87,63 @@ def test_blocks_of_the_most_rows(gpu):
     # the reciprocal (2^-23 allowed) and the last product round by 2^-24 each: 2^-21 in all.
     want = v[:, :, 16].double()
     assert bool(((out.double() - want).abs() <= 2.0 ** -21 * want.abs()).all())
+
+
+# What the terms of a 16-bit type leave of a query and of a probability, at worst: of the value itself, and of the
+# row's largest (include/ct2_mi355.h).
+QUERY_LEFT = {"f32": (0, 0), "f16": (2.0 ** -22, 2.0 ** -36), "bf16": (2.0 ** -27, 0)}
+PROBABILITY_LEFT = {"f32": (0, 0), "f16": (2.0 ** -22, 2.0 ** -38), "bf16": (2.0 ** -27, 0)}
+SPANS = [(4, 2, 64, None), (20, 8, 64, None), (20, 8, 128, None), (40, 4, 64, 380000),
+         (40, 4, 128, 380000), (2, 2, 256, None)]
+
+
+@pytest.mark.parametrize("dtype", C.TYPES)
+@pytest.mark.parametrize("tokens, heads, dhead, room", SPANS, ids=str)
+@pytest.mark.parametrize("size", (1024.0, 16384.0))
+def test_tree_one_large_query_channel(gpu, dtype, tokens, heads, dhead, room, size):
+    """A query channel far above the others, on key channels of zero: the others' products decide, and each is to be
+    as good as its own size allows.
+
+    The scores are off by ds as in tests/test_cache_ops_gpu.py, its split term among them (that formula counts terms
+    relative to each element), and by what is left of the largest element's size times the keys' 1-norm."""
+    gen, rng = C.generator(44), np.random.default_rng(44)
+    n = 300
+    k, v = C.make_cache(gen, dtype, 1, 1, room or n + tokens, dhead)
+    k[..., 5] = 0
+    q = torch.randn((1, tokens, heads, dhead), device="cuda", generator=gen) * 2
+    q[..., 5] = size
+    seen = C.tree_mask(rng, 1, tokens)
+    scale = 1 / math.sqrt(dhead)
+    got = C.run_tree(q, k, v, dtype, None, n, C.to_words(seen), scale)
+    visible = torch.ones((tokens, n + tokens), dtype=torch.bool, device="cuda")
+    visible[:, n:] = torch.from_numpy(seen[0]).cuda()
+    for h in range(heads):
+        kk, vv = k[0, 0, :n + tokens], v[0, 0, :n + tokens]
+        want, tol, _ = C.reference(q[0, :, h], kk, vv, visible, scale, dtype)
+        left = QUERY_LEFT[dtype][1] * size * scale * float(kk.double().abs().sum(1).max())
+        C.within(got[0, :, h], want, tol + 2 * left * float(vv.double().abs().max()), "head %d" % h)
+
+
+@pytest.mark.parametrize("dtype", C.TYPES)
+@pytest.mark.parametrize("tokens, heads, dhead, room", SPANS, ids=str)
+@pytest.mark.parametrize("depth", (15.3, 18.7, 20.6))
+def test_tree_a_long_tail_of_small_probabilities(gpu, dtype, tokens, heads, dhead, room, depth):
+    """Every sixteenth position takes nearly all of the probability and has values of zero: the output is the sum over
+    thousands of positions with probabilities 2^-depth of those, all alike, whose errors add up. Each is off by what
+    is left of it and of the row's largest, on top of the tolerance of tests/test_cache_ops_gpu.py."""
+    gen = C.generator(45)
+    n = 4000
+    k = torch.zeros((1, 1, room or n + tokens, dhead), dtype=C.TYPES[dtype][1], device="cuda")
+    v = torch.zeros_like(k)
+    v[0, 0, :n] = 1 + torch.rand((n, dhead), device="cuda", generator=gen)
+    k[0, 0, :n:16, 0] = 1
+    v[0, 0, :n:16] = 0
+    q = torch.zeros((1, tokens, heads, dhead), device="cuda")
+    q[..., 0] = depth * math.log(2)  # the score of those positions; the others' are zero
+    seen = np.zeros((1, tokens, tokens), dtype=bool)
+    got = C.run_tree(q, k, v, dtype, None, n, C.to_words(seen), 1.0)
+    visible = torch.ones((tokens, n), dtype=torch.bool, device="cuda")
+    for h in range(heads):
+        want, tol, p = C.reference(q[0, :, h], k[0, 0, :n], v[0, 0, :n], visible, 1.0, dtype)
+        off = PROBABILITY_LEFT[dtype][1] * float(p[0][0].max()) * v[0, 0, :n].double().sum(0)
+        C.within(got[0, :, h], want, tol + off, "head %d" % h)
