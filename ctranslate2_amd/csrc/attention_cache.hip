@@ -559,19 +559,17 @@ struct Worker {
       }
       if constexpr (kView == CacheView::kTree) {
         // a drafted position's NaN and infinite values would reach rows that do not see it as 0 x inf:
-        // they wait for add_not_finite(); those of the committed ones before it every row sees
+        // they wait for add_not_finite(), and with them those of the step's committed positions
 #pragma unroll
-        for (int j = 0; j < T::kLane; ++j) {
-          const bool drafted = at + j >= len;
+        for (int j = 0; j < T::kLane; ++j)
 #pragma unroll
           for (int h = 0; h < T::H; ++h)
 #pragma unroll
             for (int w = 0; w < T::kWords; ++w) {
-              const uint32_t x = drafted ? finite_part(v[j][h][w]) : v[j][h][w];
+              const uint32_t x = finite_part(v[j][h][w]);
               not_finite |= x != v[j][h][w];
               v[j][h][w] = x;
             }
-        }
       }
     }
     if (kView == CacheView::kDense && p.weights) {
@@ -668,15 +666,17 @@ struct Worker {
     }
   }
 
-  // The NaN and infinite values of drafted positions, to the rows that see them. (A probability is above
-  // zero, so its product with them is what they are.)
+  // The NaN and infinite values that the walk took out, to the rows that see them: of the drafted positions and
+  // of the committed ones in the step that those begin in. (A probability is above zero, so its product with
+  // them is what they are.)
   __device__ void add_not_finite(int r0, int r1) {
     constexpr int kStretch = kShared ? T::kTileKeys : T::kStep;  // of a wave in a round
+    const int first = len / T::kStep * T::kStep;
 #pragma unroll 1
     for (int r = r0; r < r1; ++r) {
       const int t = (r << plan.round_shift) + wave_k * kStretch, to = t + kStretch < end ? t + kStretch : end;
 #pragma unroll 1
-      for (int at = t < len ? len : t; at < to; ++at) {
+      for (int at = t < first ? first : t; at < to; ++at) {
         bool seen[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) seen[n] = !(hidden_from(row0 + n * 16 + c, at) & 1);
