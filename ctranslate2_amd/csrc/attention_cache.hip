@@ -24,19 +24,20 @@
 // bound by the matrix cores (and, on short caches, by a workgroup's way in and out: queries split, parts
 // written and joined).
 // Measured, with finish_kernel: 32 entries of 5.2 k positions on average, 8 heads of 128 bfloat16, one
-// token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 297 us, 0.98 PFLOP/s of
-// 16-bit products, six for each of the formula's (a library product of 8192^3: 1.12); 16 entries of 1.3 k, 26
-// tokens: 54 us. Tried with two terms of bfloat16 on the second, where they and 32 rows a wave took 200 us:
+// token of 32 heads: 157 us, 4.4 TB/s (a copy: 5.06); 4 entries of 23 k, 64 tokens: 298 to 305 us, 0.95 to 0.98
+// PFLOP/s of 16-bit products, three for each of the formula's (a library product of 8192^3: 1.12); 16 entries of
+// 1.3 k, 26 tokens: 55 us. Tried with two terms of bfloat16 on the second, where they and 32 rows a wave took 200 us:
 // four row tiles per wave without LDS 452 us (outputs and queries need all 512 registers and spill), values by
 // the transposing LDS read instead of v_perm 220 against 207.
 //
 // 16-bit caches: a query (scaled by a power of two to [1, 2) first) and a probability enter as a sum of
-// 16-bit terms - the output is float32, and one term would cost 2^-9 (bfloat16) or 2^-12 (float16).
-// Three of bfloat16 leave 2^-27. float16's steps end at 2^-24, so that a second term of something small holds
+// 16-bit terms - the output is float32, and one term would cost 2^-8 (bfloat16) or 2^-11 (float16).
+// A term's rest is at most half its step, and its sign one bit more: three of bfloat16 leave 2^-26 (two 2^-17),
+// two of float16 2^-23. float16's steps end at 2^-24, so that a second term of something small holds
 // only its first bits. A query's is therefore what the first left times 2^11, with sums of its own that
-// join the others' times 2^-11: 2^-22 of an element is left, or 2^-36 of the row's largest (unscaled: 2^-25 of the
+// join the others' times 2^-11: 2^-23 of an element is left, or 2^-36 of the row's largest (unscaled: 2^-25 of the
 // row's largest; 300 positions, one query channel of 16384 beside others of 2: outputs off by 4e-4). A
-// probability's range ends below 2^16 and begins at 2^13 (kLift): 2^-22 of it is left, or 2^-38 of the row's
+// probability's range ends below 2^16 and begins at 2^13 (kLift): 2^-23 of it is left, or 2^-38 of the row's
 // largest. (Sums of their own for it as well: 5 to 15 % of a tree's time, 340 for 290 us on 16 x 64 tokens and
 // 8 k positions.)
 // float32 caches use the float32 MFMA, nothing is rounded.
@@ -226,8 +227,8 @@ struct Worker {
   const int32_t* selected;
 
   // 16-bit terms of a query and of a probability: three of bfloat16 and two of float16 carry float32. Two of
-  // bfloat16 (2^-18) and 32 rows a wave took 200 us where 16 rows and three take 305 (4 entries of 23 k, 64
-  // tokens), with an error twice that of float32 arithmetic (4.6e-6): not taken.
+  // bfloat16 (2^-17) and 32 rows a wave took 200 us where 16 rows and three take 305 (4 entries of 23 k, 64
+  // tokens), with an error twice that of float32 arithmetic (4.6e-6 against 2.1e-6; three: 9.8e-7): not taken.
   static constexpr int kTerms = !T::kHalf ? 1 : kType == kBF16 ? 3 : 2;
   static constexpr bool kApart = kType == kF16;  // the products of the queries' second terms have sums of their own
   static constexpr float kBack = kApart ? 1.f / 2048 : 1.f;  // and this factor
@@ -1071,7 +1072,9 @@ CachePlan make_plan(const CacheAttnParams& p) {
   // 192 units, less than 512 and more; heads of 128, us, line / alone, units and positions (bfloat16):
   // tree 4 tokens, 64 x 512: 14.1 / 13.4, 192 x 1020: 30.0 / 22.0, 512 x 2044: 70.8 / 63.4; 24 tokens,
   // 64 x 1020: 31 / 48, 512 x 1532: 146 / 120; blocks 64 x 1024: 29 / 41, 512 x 1024: 76 / 74;
-  // accumulate 192 x 250: 15.2 / 13.3, 512 x 1000: 39 / 36.
+  // accumulate 192 x 250: 15.2 / 13.3, 512 x 1000: 39 / 36. (Entries without a figure of their own lie between
+  // those of their row.) Lengths are not known here, t_max is: a cache with much more room than its entries fill
+  // gets the line.
   static constexpr int kAlone[3][3] = {{2, 8, 16}, {2, 4, 32}, {8, 16, 32}};
   const int many = units >= 512 ? 2 : units >= 192 ? 1 : 0;
   const int view = p.view == CacheView::kDense ? 0 : p.view == CacheView::kBlocks ? 1 : 2;

@@ -542,8 +542,8 @@ int ct2x_attention_full_half(const float* d_q, const float* d_k, const float* d_
  * (clamped to what the cache holds), or `length` where d_lengths is NULL (`length` is not read
  * otherwise). What lies behind an entry's positions is never looked at: it may hold anything.
  * Scores, softmax statistics and sums are fp32. Products with 16-bit caches run on the 16-bit matrix
- * cores, the fp32 operand (query, probability) as a sum of 16-bit terms: three of bfloat16 (2^-27 of it
- * left), two of float16 (2^-22 of it left, or of a query 2^-36 of its row's largest element, of a probability 2^-38
+ * cores, the fp32 operand (query, probability) as a sum of 16-bit terms: three of bfloat16 (2^-26 of it
+ * left), two of float16 (2^-23 of it left, or of a query 2^-36 of its row's largest element, of a probability 2^-38
  * of its row's largest, if that is more). What a row sees is to be finite: an infinite or NaN query, key or
  * value leaves infinities or NaN in the rows that see it. A row that sees nothing gets an output of zero.
  * d_scratch: at least the *_scratch_bytes() of the same sizes (-1: the sizes are refused, see

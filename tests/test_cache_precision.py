@@ -7,8 +7,8 @@ exponents' arguments up to about 12 x log2(e) and rounded at 2^-24 of that, twic
 up to 256 products round at 2^-24 of what they hold, some ten times; the exponential, the terms and the last sums add
 a few times 2^-24. All of them have independent signs, so that their squares add up: between 5 and 15 x 2^-24 for a
 probability, and a sum over many of them is off by no more, relatively. Two terms of bfloat16 instead of three leave
-2^-18 of every query element and probability (a quarter of that on average): 2^-20 x (2 of the score's size, 1) = 36
-x 2^-24 in the square's mean, which the bound tells apart (the last test, in float64).
+2^-17 of every query element and probability at worst, a quarter of that in the square's mean: 2^-19 x (2 of the
+score's size, 1) = 71 x 2^-24, which the bound tells apart (the last test, in float64).
 
 float32 caches have no terms to tell apart, and a rounding for every product instead of one for 32: a rounding is off
 by 0.41 x 2^-24 of the partial sum in the square's mean (half a step, evenly spread over a step and over the step's
