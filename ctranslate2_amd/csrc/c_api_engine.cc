@@ -1228,6 +1228,7 @@ static int translate_batch_impl(void* translator, const int32_t* src_ids,
   }
   streams = std::max<int32_t>(1, std::min<int32_t>(streams, 16));
   if (t->engine->profiling()) streams = 1;  // event bookkeeping is single-stream
+  if (t->engine->tp_world() > 1) streams = 1;  // (the ranks' exchanges meet in the order of one session)
   if (dopt.callback) streams = 1;           // the callback is called from one thread
   const size_t ref_chunk = opt.max_batch_size > 0 ? static_cast<size_t>(opt.max_batch_size)
                                                   : std::max<size_t>(order.size(), 1);

@@ -669,7 +669,7 @@ struct ct2x_translation_options {
   int32_t num_streams;          /* >1: split the batch into independent sub-batches decoded
                                    concurrently on separate HIP streams of the SAME GPU (the
                                    reference's several replicas per device, replica_pool.h:243-260);
-                                   0 = choose automatically */
+                                   0 = choose automatically; tensor-parallel ranks: 1 */
   /* RandomSampler (src/sampling.cc:41-101; python: sampling_topk / sampling_topp /
    * sampling_temperature), greedy search (beam_size 1) only. sampling_topk: 1 = arg-max
    * (BestSampler), k >= 2 = sample among the best k, -1 = sample from the whole vocabulary (the

@@ -119,3 +119,29 @@ def test_give_up_needs_mailboxes(gpu):
         with pytest.raises(ct2.Ct2xError, match="tensor-parallel rank|no mailboxes"):
             t.debug_give_up_exchanges()
         t.close()
+
+
+def test_streams_asked_of_a_rank_are_one(gpu):
+    """num_streams splits a batch into sessions that run at once; a rank's exchanges meet the others' in the order of
+    one session, so a tensor-parallel rank takes the sub-batches together."""
+    import ctranslate2_amd as ct2
+    path, cfg, src = _model_dir("tiny"), GC.SYNTHETIC["tiny"], _sources("tiny")
+    kw = dict(beam_size=2, max_decoding_length=cfg["max_len"], min_decoding_length=cfg["min_len"],
+              return_scores=True, num_streams=3)
+    single = ct2.Translator(path, compute_type="int8")
+    want, scores = single.translate_ids(src, **kw)
+    ranks = ct2.Translator.tensor_parallel_local(path, 2, compute_type="int8")
+    got = [None, None]
+
+    def work(r):
+        got[r] = ranks[r].translate_ids(src, **kw)
+
+    threads = [threading.Thread(target=work, args=(r,)) for r in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=90)
+    for hyps, s in got:
+        assert hyps == want and np.array_equal(s, scores)
+    for t in ranks:
+        t.close()
