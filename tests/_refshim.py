@@ -5,6 +5,7 @@ Used to pin the C restatement oracle, to generate tests/golden fixtures and to t
 import ctypes as C
 import glob
 import os
+import sys
 
 import numpy as np
 
@@ -27,6 +28,8 @@ def lib():
     global _lib
     if _lib is not None:
         return _lib
+    if not available() and "pytest" in sys.modules:  # what compares with the reference has nothing to compare with
+        sys.modules["pytest"].skip("oracle/_ref (the compiled reference) is not present")
     # The reference selects MKL only on GenuineIntel CPUs unless told otherwise
     # (src/cpu/backend.cc:10-31); the GPU box has AMD EPYC host cores.
     os.environ.setdefault("CT2_USE_MKL", "1")
