@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdlib>
+#include <filesystem>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -21,6 +22,24 @@ struct Vml {
   VmlFn vs_sin = nullptr;
   VmlFn vs_cos = nullptr;
 };
+
+// libmkl_rt loads the rest of MKL when it is first called, and ends the process where that is missing: it is
+// used only if core, threading layer and vector functions lie beside it.
+bool complete(const void* symbol) {
+  Dl_info info;
+  if (dladdr(symbol, &info) == 0 || info.dli_fname == nullptr) return false;
+  std::error_code error;
+  const std::filesystem::path file = std::filesystem::canonical(info.dli_fname, error);
+  if (error) return false;
+  bool core = false, threads = false, vml = false;
+  for (const auto& entry : std::filesystem::directory_iterator(file.parent_path(), error)) {
+    const std::string name = entry.path().filename().string();
+    core = core || name.rfind("libmkl_core.so", 0) == 0;
+    threads = threads || name.rfind("libmkl_intel_thread.so", 0) == 0;
+    vml = vml || name.rfind("libmkl_vml_", 0) == 0;
+  }
+  return core && threads && vml;
+}
 
 Vml& vml() {
   static Vml v;
@@ -40,21 +59,20 @@ Vml& vml() {
     dirs.push_back("/opt/conda/lib/");
     dirs.push_back("/opt/intel/oneapi/mkl/latest/lib/");
     dirs.push_back("/opt/intel/oneapi/mkl/latest/lib/intel64/");
-    void* h = nullptr;
-    for (const auto& d : dirs) {
+    for (const auto& d : dirs)
       for (const char* name : {"libmkl_rt.so.2", "libmkl_rt.so.1", "libmkl_rt.so"}) {
-        h = dlopen((d + name).c_str(), RTLD_LAZY | RTLD_LOCAL);
-        if (h) break;
+        void* h = v.vs_sin ? nullptr : dlopen((d + name).c_str(), RTLD_LAZY | RTLD_LOCAL);
+        if (!h) continue;
+        // (no MKL_Set_Threading_Layer here: the library may be shared with the host application -
+        // numpy's, say - and the threading layer is process wide)
+        void *sin = dlsym(h, "vsSin"), *cos = dlsym(h, "vsCos");
+        if (sin && cos && complete(sin)) {
+          v.vs_sin = reinterpret_cast<VmlFn>(sin);
+          v.vs_cos = reinterpret_cast<VmlFn>(cos);
+        } else {
+          (void)dlclose(h);
+        }
       }
-      if (h) break;
-    }
-    if (h) {
-      // (no MKL_Set_Threading_Layer here: the library may be shared with the host application -
-      // numpy's, say - and the threading layer is process wide)
-      v.vs_sin = reinterpret_cast<VmlFn>(dlsym(h, "vsSin"));
-      v.vs_cos = reinterpret_cast<VmlFn>(dlsym(h, "vsCos"));
-      if (!v.vs_sin || !v.vs_cos) v.vs_sin = v.vs_cos = nullptr;
-    }
     if (want == "mkl" && !v.vs_sin)
       throw std::runtime_error("CT2X_HOST_MATH=mkl but no MKL runtime (libmkl_rt.so) was found; set "
                                "CT2X_MKL_PATH");

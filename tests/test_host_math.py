@@ -53,3 +53,23 @@ def test_host_sin_cos_within_an_ulp(kind):
     s, c = host_sin_cos(x)
     for got, want in ((s, np.sin(x.astype(np.float64))), (c, np.cos(x.astype(np.float64)))):
         assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want) + 1e-40)
+
+
+def test_a_partial_mkl_is_passed_over(tmp_path):
+    """libmkl_rt alone, without the libraries that it loads when it is called, ends a process: it is not used."""
+    import glob
+    import os
+    import shutil
+    import subprocess
+    import sys
+    rt = sorted(glob.glob("/opt/conda/lib/libmkl_rt.so*"))
+    if not rt:
+        pytest.skip("no MKL runtime")
+    shutil.copy(rt[0], tmp_path / "libmkl_rt.so.1")
+    code = ("import sys; sys.path[:0] = %r; import numpy as np, test_host_math as T; "
+            "x = np.array([0.5, 2.0], np.float32); s, c = T.host_sin_cos(x); "
+            "assert abs(s - np.sin(x)).max() < 1e-6; print('BACKEND', T.backend())" %
+            [os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))])
+    env = dict(os.environ, CT2X_MKL_PATH=str(tmp_path))
+    p = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0 and "BACKEND" in p.stdout, p.stderr[-2000:]
